@@ -161,6 +161,27 @@ class PlanStats(C.Structure):
         return {k: getattr(self, k) for k, _ in self._fields_}
 
 
+# element types of readout rows (hx_dtype)
+HX_DT = {"f64": 0, "f32": 1, "f16": 2, "bf16": 3}
+
+
+class Readout(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("dtype", C.c_int), ("nrow", C.c_int), ("ncol", C.c_int), ("ld", C.c_longlong)]
+
+
+class Teacher(C.Structure):
+    _fields_ = [("idx", C.c_void_p), ("val", C.c_void_p), ("lse", C.c_void_p), ("dtype", C.c_int), ("k", C.c_int)]
+
+
+class SampleRule(C.Structure):
+    _fields_ = [("temperature", C.c_double), ("top_k", C.c_double), ("top_p", C.c_double), ("min_p", C.c_double)]
+
+
+_top_args = [C.POINTER(Readout), C.c_int, C.c_double, C.c_void_p, C.c_void_p, C.c_void_p]
+_distill_args = [C.POINTER(Readout), C.POINTER(Teacher), C.c_double, C.c_double, C.c_void_p, C.c_void_p, C.c_longlong,
+                 C.c_void_p, C.c_void_p]
+_sample_args = [C.POINTER(Readout), C.POINTER(SampleRule), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "hx_abi_version": (C.c_int, []),
@@ -191,6 +212,12 @@ SIGNATURES = {
     "hx_mse_loss_grad_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p]),
     "hx_mse_loss_grad_noalloc": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p,
                                             C.c_void_p]),
+    "hx_top_logits_dev": (C.c_int, [C.c_void_p] + _top_args),
+    "hx_distill_loss_grad_dev": (C.c_int, [C.c_void_p] + _distill_args),
+    "hx_sample_dev": (C.c_int, [C.c_void_p] + _sample_args),
+    "hx_top_logits_check": (C.c_int, _top_args + [C.c_char_p, C.c_int]),
+    "hx_distill_check": (C.c_int, _distill_args + [C.c_char_p, C.c_int]),
+    "hx_sample_check": (C.c_int, _sample_args + [C.c_char_p, C.c_int]),
     "hx_last_kernel_ms": (C.c_int, [C.c_void_p, C.c_int, _dp, _ip]),
     "hx_rcp_nz_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
     "hx_opt_create_adam": (C.c_int, [C.c_void_p, C.c_double, C.c_double, C.c_double]),

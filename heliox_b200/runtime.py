@@ -79,6 +79,16 @@ def _out_array(out: Optional[np.ndarray], shape) -> np.ndarray:
     return out
 
 
+def _dt(dtype: str) -> int:
+    if dtype not in _lib.HX_DT:
+        raise ValueError(f"dtype must be one of {sorted(_lib.HX_DT)} (got {dtype!r})")
+    return _lib.HX_DT[dtype]
+
+
+def _readout(ptr: int, nrow: int, ncol: int, dtype: str, ld: Optional[int]) -> "_lib.Readout":
+    return _lib.Readout(int(ptr) or None, _dt(dtype), int(nrow), int(ncol), int(ncol if ld is None else ld))
+
+
 class Sim:
     """One simulation/learning runtime bound to one CUDA device."""
 
@@ -364,6 +374,59 @@ class Sim:
         self._check(self._L.hx_mse_loss_grad_dev(self._ctx, C.c_void_p(int(trace_ptr)), C.c_void_p(int(target_ptr)),
                                                  int(nrow), int(ncol), C.c_void_p(int(dLdv_ptr)),
                                                  C.c_void_p(int(loss_ptr))), "hx_mse_loss_grad_dev")
+
+    # ------------------------------------------------------------------ readout rows (device pointers)
+    def top_logits_dev(self, logits_ptr: int, nrow: int, ncol: int, k: int, idx_ptr: int, val_ptr: int, *,
+                       lse_ptr: int = 0, temperature: float = 1.0, dtype: str = "f64", ld: Optional[int] = None):
+        """The k largest readouts of each row with their positions, in descending
+        order, and the rows' log-sum-exp at ``temperature``: a teacher's record.
+
+        ``logits_ptr``: nrow x ncol readouts of ``dtype`` ("f64", "f32", "f16",
+        "bf16"), rows ``ld`` elements apart (default: ncol); ``idx_ptr``: nrow x
+        k int32; ``val_ptr``: nrow x k of ``dtype``; ``lse_ptr``: nrow values
+        (float64 for "f64" rows, else float32), 0 to leave them out."""
+        rows = _readout(logits_ptr, nrow, ncol, dtype, ld)
+        self._check(self._L.hx_top_logits_dev(self._ctx, C.byref(rows), int(k), float(temperature),
+                                              C.c_void_p(int(idx_ptr)), C.c_void_p(int(val_ptr)),
+                                              C.c_void_p(int(lse_ptr))), "hx_top_logits_dev")
+
+    def distill_loss_grad_dev(self, logits_ptr: int, nrow: int, ncol: int, k: int, t_idx_ptr: int, t_val_ptr: int,
+                              grad_ptr: int, row_loss_ptr: int, loss_ptr: int, *, t_lse_ptr: int = 0,
+                              temperature: float = 1.0, scale: Optional[float] = None, row_weight_ptr: int = 0,
+                              dtype: str = "f64", t_dtype: Optional[str] = None, ld: Optional[int] = None,
+                              ld_grad: Optional[int] = None):
+        """Loss of a student's rows against a teacher's record (``top_logits_dev``)
+        and its gradient with respect to every readout.
+
+        ``t_lse_ptr`` 0: the teacher's probabilities are renormalised over its
+        slots; otherwise the rest of each row counts as one more class.
+        ``grad_ptr`` may be ``logits_ptr`` (in place) or 0 (loss only);
+        ``row_loss_ptr``: nrow values, ``loss_ptr``: one (float64 for "f64"
+        rows, else float32).  ``scale`` defaults to 1 / nrow (the mean over
+        rows); ``row_weight_ptr``: nrow float64 weights, 0 for ones."""
+        rows = _readout(logits_ptr, nrow, ncol, dtype, ld)
+        t = _lib.Teacher(int(t_idx_ptr), int(t_val_ptr), int(t_lse_ptr) or None, _dt(t_dtype or dtype), int(k))
+        sc = (1.0 / nrow if nrow > 0 else 1.0) if scale is None else float(scale)
+        self._check(self._L.hx_distill_loss_grad_dev(
+            self._ctx, C.byref(rows), C.byref(t), float(temperature), sc, C.c_void_p(int(row_weight_ptr)),
+            C.c_void_p(int(grad_ptr)), int(ncol if ld_grad is None else ld_grad), C.c_void_p(int(row_loss_ptr)),
+            C.c_void_p(int(loss_ptr))), "hx_distill_loss_grad_dev")
+
+    def sample_dev(self, logits_ptr: int, nrow: int, ncol: int, u_ptr: int, idx_ptr: int, *, logp_ptr: int = 0,
+                   temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
+                   rules_ptr: int = 0, dtype: str = "f64", ld: Optional[int] = None):
+        """One choice per row from the uniform numbers at ``u_ptr`` (nrow float64 in [0, 1)).
+
+        ``idx_ptr``: nrow int32 positions (-1: a row without an open readout,
+        -2: NaN or +inf in it); ``logp_ptr``: nrow log-probabilities within what
+        the rule leaves (float64 for "f64" rows, else float32), 0 to leave them
+        out.  ``rules_ptr``: nrow x 4 float64 on the device (temperature, top_k,
+        top_p, min_p of each row) in place of the four arguments."""
+        rows = _readout(logits_ptr, nrow, ncol, dtype, ld)
+        rule = _lib.SampleRule(float(temperature), float(top_k), float(top_p), float(min_p))
+        self._check(self._L.hx_sample_dev(self._ctx, C.byref(rows), C.byref(rule), C.c_void_p(int(rules_ptr)),
+                                          C.c_void_p(int(u_ptr)), C.c_void_p(int(idx_ptr)),
+                                          C.c_void_p(int(logp_ptr))), "hx_sample_dev")
 
     # ------------------------------------------------------------------ optimizer
     # Mirrors Sim.create_optimizer / configure_optimizer / optimizer_add_external_grads /

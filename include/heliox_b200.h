@@ -530,6 +530,115 @@ int hx_mse_loss_grad_dev(hx_ctx* ctx, const double* trace_dev, const double* tar
 int hx_mse_loss_grad_noalloc(const double* trace_dev, const double* target_dev, int nrow, int ncol, double* dLdv_dev,
                              double* loss_dev, void* stream);
 
+/* ---- readout rows ----------------------------------------------------------------- */
+/* A probe trace is a matrix of readouts: one row per step, one column per
+ * probe.  The entries below train a network to choose among its readouts as a
+ * teacher does, and take its choices.  They also take rows of other types, so
+ * that the teacher may be another model (fp32, fp16 or bf16 logits).
+ * Pointers inside the descriptors are device pointers on the context's device.
+ * The work is enqueued on the context's stream; the entries allocate nothing,
+ * keep no state between calls and may be captured into CUDA graphs.  Results
+ * do not depend on how the work is split or timed: two calls on the same
+ * inputs give the same bits.  A -inf readout is a closed choice: it has
+ * probability 0 and is never taken.  "Statistics" (log-sum-exp, losses,
+ * log-probabilities) are double for HX_DT_F64 rows and float for the others.
+ * The reference has no counterpart (its objectives are Python callables on the
+ * output trace, python_lib/heliox_learn/objective.py:15-30). */
+enum hx_dtype { HX_DT_F64 = 0, HX_DT_F32 = 1, HX_DT_F16 = 2, HX_DT_BF16 = 3 };
+
+/* Columns a row may have, and slots of a teacher's record. */
+#define HX_READOUT_MAX_ROW_BYTES 1572864
+#define HX_READOUT_MAX_K 1024
+
+/* nrow rows of ncol readouts, row r at x + r * ld (ld >= ncol, in elements;
+ * ncol times the element size at most HX_READOUT_MAX_ROW_BYTES). */
+typedef struct hx_readout {
+    const void* x;
+    int dtype; /* hx_dtype */
+    int nrow, ncol;
+    long long ld;
+} hx_readout;
+
+/* A teacher's record of the same rows, as hx_top_logits_dev writes it: k slots
+ * a row (nrow x k): the readout's position and its value.  A position outside
+ * 0 .. ncol-1 or a value of -inf marks an unused slot; where a position comes
+ * twice in a row the lower slot counts.  lse (nrow statistics of the teacher's
+ * type, or NULL): the log-sum-exp of the teacher's whole row at the
+ * temperature of the loss. */
+typedef struct hx_teacher {
+    const int32_t* idx;
+    const void* val;
+    const void* lse;
+    int dtype; /* of val: hx_dtype */
+    int k;     /* 1 .. HX_READOUT_MAX_K */
+} hx_teacher;
+
+/* How a choice is drawn (four doubles; a device array of them is a plain nrow
+ * x 4 matrix).  temperature > 0 divides the readouts; 0 takes the largest.
+ * top_k: only the top_k largest (rounded down; below 1: all).  top_p: only the
+ * shortest run of the largest that holds at least this share of what top_k
+ * left (1: all).  min_p: only those at least this many times as probable as
+ * the most probable (0: all). */
+typedef struct hx_sample_rule {
+    double temperature, top_k, top_p, min_p;
+} hx_sample_rule;
+
+/* The k largest readouts of each row, in descending order (equal ones: the
+ * lower position first): idx_dev (nrow x k) their positions, val_dev (nrow x k,
+ * of the rows' type) their values.  Slots beyond the row's readouts above -inf
+ * get -1 and -inf.  lse_dev (nrow statistics, may be NULL): log sum_i
+ * exp(x_i / temperature), -inf for a row without an open readout.  A row that
+ * holds a NaN gets positions -1, values and log-sum-exp NaN. */
+int hx_top_logits_dev(hx_ctx* ctx, const hx_readout* rows, int k, double temperature, int32_t* idx_dev, void* val_dev,
+                      void* lse_dev);
+
+/* Loss of the rows against a teacher's record, and its gradient.  With p =
+ * softmax(x / T) over the row and v the used slots' values:
+ *   teacher->lse NULL: q = softmax(v / T) over the used slots,
+ *     L = T^2 sum_j q_j (log q_j - log p_j),     dL/dx_i = T (p_i - q_i)
+ *     (one slot: the cross entropy with that label, times T^2);
+ *   else: q_j = exp(v_j / T - lse), and the rest of the row is one more class,
+ *     q_r = max(0, 1 - sum q_j), p_r = sum of p outside the slots,
+ *     L = T^2 (sum_j q_j (log q_j - log p_j) + q_r (log q_r - log p_r)),
+ *     dL/dx_i = T (Q p_i - q_i) in a slot and T p_i (Q - q_r / p_r) outside,
+ *     Q = sum q_j + q_r; a term whose q is 0, or whose p_r is 0, is left out.
+ * row_loss_dev[r] = L_r; *loss_dev = scale * sum_r w_r L_r, with w =
+ * row_weight_dev (nrow doubles) or 1; grad_dev (rows' type, row r at
+ * grad_dev + r * ld_grad; may be NULL, or the rows' own memory with the same
+ * ld) = scale * w_r dL_r/dx, each rounded once.  Rows of weight 0 are not read;
+ * they, rows without a used slot and rows without an open readout get a loss
+ * of 0 and gradients of 0.  NaN, or +inf, in another row gives NaN there.
+ * loss_dev and row_loss_dev: statistics of the rows' type. */
+int hx_distill_loss_grad_dev(hx_ctx* ctx, const hx_readout* rows, const hx_teacher* teacher, double temperature,
+                             double scale, const double* row_weight_dev, void* grad_dev, long long ld_grad,
+                             void* row_loss_dev, void* loss_dev);
+
+/* One choice per row from the uniform numbers u_dev (nrow doubles in [0, 1)).
+ * The row's readouts in descending order (equal ones: the lower position
+ * first) are cut to the shortest run that *rule, or rules_dev[r] (nrow rules on
+ * the device; rule is then not read and may be NULL), leaves; the choice is the
+ * first whose running probability exceeds u times that of the run.
+ * idx_dev[r]: its position, -1 for a row without an open readout, -2 for a row
+ * that holds NaN or +inf or whose rule's temperature is NaN.  logp_dev (nrow
+ * statistics, may be NULL): the log of its probability within the run (-inf and
+ * NaN beside -1 and -2).  Probabilities count in units of 2^-s of the largest
+ * one, s = min(52, 62 - log2 ncol rounded up).  In rules_dev a temperature
+ * below or at 0 takes the largest, a share top_p outside (0, 1) is 1 above and
+ * leaves the largest alone below, min_p is held to [0, 1], NaN in the three
+ * switches that cut off; u outside [0, 1) is held to it, NaN is 0. */
+int hx_sample_dev(hx_ctx* ctx, const hx_readout* rows, const hx_sample_rule* rule, const hx_sample_rule* rules_dev,
+                  const double* u_dev, int32_t* idx_dev, void* logp_dev);
+
+/* The three entries' checks of their arguments, on the host only (no device
+ * needed): 0, or -1 with the reason in msg (at most cap bytes, NULL allowed). */
+int hx_top_logits_check(const hx_readout* rows, int k, double temperature, const int32_t* idx_dev, const void* val_dev,
+                        const void* lse_dev, char* msg, int cap);
+int hx_distill_check(const hx_readout* rows, const hx_teacher* teacher, double temperature, double scale,
+                     const double* row_weight_dev, const void* grad_dev, long long ld_grad, const void* row_loss_dev,
+                     const void* loss_dev, char* msg, int cap);
+int hx_sample_check(const hx_readout* rows, const hx_sample_rule* rule, const hx_sample_rule* rules_dev,
+                    const double* u_dev, const int32_t* idx_dev, const void* logp_dev, char* msg, int cap);
+
 /* ---- verification -------------------------------------------------------------- */
 /* y[i] = the reciprocal the step kernels use in place of IEEE division in the
  * mechanism rate functions (hardware estimate + two Newton-Raphson steps), for
