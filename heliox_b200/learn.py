@@ -201,3 +201,130 @@ def train_adam(runtime: AdjointRuntime, handles: Sequence[int], target: np.ndarr
             on_epoch(ep, loss)
     sim.synchronize()
     return hist
+
+
+@dataclass
+class TeacherRecord:
+    """A teacher's top readouts of the steps 1..T of a trial (device tensors):
+    what ``train_distill`` fits a student to."""
+
+    idx: Any  # int32 (T, k): probe columns in descending order, -1 where unused
+    val: Any  # float64 (T, k): their voltages
+    lse: Any  # float64 (T,) log-sum-exp of the whole row at ``temperature``, or None
+    ncol: int
+    temperature: float
+
+    @property
+    def total_steps(self) -> int:
+        return int(self.idx.shape[0])
+
+    @property
+    def k(self) -> int:
+        return int(self.idx.shape[1])
+
+
+def _device_trace(runtime: AdjointRuntime, total_steps: int, ncol: int):
+    """A zeroed (T+1, ncol) float64 buffer on the runtime's device, safe to use on the runtime's stream."""
+    import torch
+
+    dev = torch.device("cuda", runtime.sim.device)
+    buf = torch.zeros((int(total_steps) + 1, int(ncol)), dtype=torch.float64, device=dev)
+    torch.cuda.current_stream(dev).synchronize()
+    return buf
+
+
+def record_teacher(runtime: AdjointRuntime, total_steps: int, k: int, temperature: float = 1.0, rest: bool = True,
+                   probes: Optional[Sequence[int]] = None) -> TeacherRecord:
+    """Run a teacher and keep the ``k`` largest readouts of every step.
+
+    The probes are the choices: step t's probabilities are softmax(v[t] /
+    temperature) (temperature in mV).  ``rest`` also keeps each row's
+    log-sum-exp, so that the loss counts what the k readouts leave out as one
+    more class; without it the k are renormalised.  A full float64 trace of
+    10,000 probes over 8,000 steps is 640 MB, 64 readouts of each step 6 MB."""
+    import torch
+
+    sim = runtime.sim
+    p = runtime.group.soma_nodes() if probes is None else np.asarray(probes, dtype=np.int32)
+    T, n = int(total_steps), int(len(p))
+    trace = _device_trace(runtime, T, n)
+    idx = torch.empty((T, int(k)), dtype=torch.int32, device=trace.device)
+    val = torch.empty((T, int(k)), dtype=torch.float64, device=trace.device)
+    lse = torch.empty(T, dtype=torch.float64, device=trace.device) if rest else None
+    sim.forward_capture_dev(T, trace.data_ptr(), probes=p)
+    sim.top_logits_dev(trace[1:].data_ptr(), T, n, int(k), idx.data_ptr(), val.data_ptr(),
+                       lse_ptr=0 if lse is None else lse.data_ptr(), temperature=temperature)
+    sim.synchronize()
+    return TeacherRecord(idx, val, lse, n, float(temperature))
+
+
+def train_distill(runtime: AdjointRuntime, handles: Sequence[int], teacher: TeacherRecord, epochs: int,
+                  lr: float = 1e-3, probes: Optional[Sequence[int]] = None, row_weight: Optional[np.ndarray] = None,
+                  allreduce: Optional[Callable[[int, int, int], None]] = None,
+                  on_epoch: Optional[Callable[[int, float], None]] = None) -> List[float]:
+    """Fit the parameters behind ``handles`` so that the probes choose as the teacher's do.
+
+    ``train_adam`` with the distillation loss in place of the trace's MSE, the
+    mean over the teacher's steps: forward capture, loss and gradient, reverse
+    sweep and Adam all stay on the device.  ``row_weight`` (T): the weight of
+    each step, 0 leaves one out.  Returns the loss history."""
+    import torch
+
+    sim = runtime.sim
+    p = runtime.group.soma_nodes() if probes is None else np.asarray(probes, dtype=np.int32)
+    T, n = teacher.total_steps, teacher.ncol
+    if len(p) != n:
+        raise ValueError(f"the teacher's record has {n} readouts a step, the student {len(p)} probes")
+    if row_weight is not None and np.shape(row_weight) != (T,):
+        raise ValueError(f"row_weight must have shape ({T},)")
+    trace, dLdv = _device_trace(runtime, T, n), _device_trace(runtime, T, n)  # row 0, the initial state, has no loss
+    if teacher.idx.device != trace.device:
+        raise ValueError(f"the teacher's record is on {teacher.idx.device}, the student on {trace.device}")
+    row_loss = torch.empty(T, dtype=torch.float64, device=trace.device)
+    losses = torch.zeros(max(int(epochs), 1), dtype=torch.float64, device=trace.device)
+    w = None if row_weight is None else torch.from_numpy(np.ascontiguousarray(row_weight, dtype=np.float64)).to(trace.device)
+    torch.cuda.current_stream(trace.device).synchronize()
+    opt = sim.create_optimizer("adam")
+    sim.optimizer_add_external_grads(opt, list(handles), impedance=1.0)
+    if allreduce is not None:
+        sim.optimizer_set_allreduce(opt, allreduce)
+    for ep in range(int(epochs)):
+        sim.forward_capture_dev(T, trace.data_ptr(), probes=p)
+        sim.distill_loss_grad_dev(trace[1:].data_ptr(), T, n, teacher.k, teacher.idx.data_ptr(), teacher.val.data_ptr(),
+                                  dLdv[1:].data_ptr(), row_loss.data_ptr(), losses[ep:].data_ptr(),
+                                  t_lse_ptr=0 if teacher.lse is None else teacher.lse.data_ptr(),
+                                  temperature=teacher.temperature, row_weight_ptr=0 if w is None else w.data_ptr())
+        sim.backward_dev(dLdv.data_ptr(), {})
+        sim.optimizer_grads_from_backward(opt)
+        sim.optimizer_step_with_inv_record_steps(opt, lr, 1.0)
+        if on_epoch:
+            sim.synchronize()
+            on_epoch(ep, float(losses[ep]))
+    sim.synchronize()
+    return [float(x) for x in losses[:int(epochs)].cpu()]
+
+
+def sample_choices(runtime: AdjointRuntime, total_steps: int, u: np.ndarray, temperature: float = 1.0, top_k: int = 0,
+                   top_p: float = 1.0, min_p: float = 0.0, probes: Optional[Sequence[int]] = None) -> Tuple[np.ndarray, np.ndarray]:
+    """Run the network and draw one choice among its probes at each of the last
+    len(u) steps, from the uniform numbers ``u``: (probe columns int32,
+    log-probabilities float64)."""
+    import torch
+
+    sim = runtime.sim
+    p = runtime.group.soma_nodes() if probes is None else np.asarray(probes, dtype=np.int32)
+    T, n = int(total_steps), int(len(p))
+    uu = np.ascontiguousarray(u, dtype=np.float64)
+    m = int(uu.shape[0])
+    if uu.ndim != 1 or m > T:
+        raise ValueError(f"u must be one-dimensional with at most {T} entries")
+    trace = _device_trace(runtime, T, n)
+    ud = torch.from_numpy(uu).to(trace.device)
+    idx = torch.empty(m, dtype=torch.int32, device=trace.device)
+    logp = torch.empty(m, dtype=torch.float64, device=trace.device)
+    torch.cuda.current_stream(trace.device).synchronize()
+    sim.forward_capture_dev(T, trace.data_ptr(), probes=p)
+    sim.sample_dev(trace[T + 1 - m:].data_ptr(), m, n, ud.data_ptr(), idx.data_ptr(), logp_ptr=logp.data_ptr(),
+                   temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+    sim.synchronize()
+    return idx.cpu().numpy(), logp.cpu().numpy()
