@@ -2,64 +2,28 @@
 // distillation loss of a student's rows with its gradient, sampled choices.
 //
 // One thread block per row; the row is read from global memory once per pass.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <climits>
 #include <cmath>
 #include <cstdio>
 #include <string>
+#include <type_traits>
 
 #include "heliox_b200.h"
 #include "hx_ctx.hpp"
+#include "hx_readout.cuh"
 
 namespace {
 
+using namespace hxr;
+
 constexpr int kThreads = 256;
 
-// Compute and statistics type W and the order-preserving integer key of each
-// element type (equal values, +0 and -0 among them, have equal keys).
-__device__ __forceinline__ unsigned long long key_of(double x) {
-    const unsigned long long b = (unsigned long long)__double_as_longlong(x + 0.0);
-    return b ^ ((b >> 63) ? ~0ull : 0x8000000000000000ull);
-}
-__device__ __forceinline__ double value_of(unsigned long long k) {
-    return __longlong_as_double((long long)(k ^ ((k >> 63) ? 0x8000000000000000ull : ~0ull)));
-}
-__device__ __forceinline__ unsigned key_of(float x) {
-    const unsigned b = __float_as_uint(x + 0.0f);
-    return b ^ ((b >> 31) ? ~0u : 0x80000000u);
-}
-__device__ __forceinline__ float value_of(unsigned k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : ~0u)); }
-
-template <typename T>
-struct Ty {  // float, __half, __nv_bfloat16
-    using W = float;
-    using K = unsigned;
-};
-template <>
-struct Ty<double> {
-    using W = double;
-    using K = unsigned long long;
-};
-
-__device__ __forceinline__ double wide(double x) { return x; }
-__device__ __forceinline__ float wide(float x) { return x; }
-__device__ __forceinline__ float wide(__half x) { return __half2float(x); }
-__device__ __forceinline__ float wide(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ void put(double* p, double v) { *p = v; }
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-
-__device__ __forceinline__ double load_any(const void* p, int dtype, size_t i) {
-    switch (dtype) {
-        case HX_DT_F64: return ((const double*)p)[i];
-        case HX_DT_F32: return (double)((const float*)p)[i];
-        case HX_DT_F16: return (double)__half2float(((const __half*)p)[i]);
-        default: return (double)__bfloat162float(((const __nv_bfloat16*)p)[i]);
-    }
-}
 
 template <typename V, typename F>
 __device__ V block_reduce(V v, V* red, F op) {  // the same order whatever the timing
@@ -239,117 +203,209 @@ __global__ void __launch_bounds__(kThreads) top_kernel(const T* __restrict__ xs,
 }
 
 // ---------------------------------------------------------------- distillation
+//
+// One pass over memory: the row waits in shared memory while its maximum, the
+// sum of its exponentials and then the gradient are taken.  The slots' readouts
+// are lifted out of the row first (-inf stands in their places), so that the
+// sum over the rest is a sum of its own and not a difference.  The teacher's
+// side is worked out while the row is on its way.
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) distill_kernel(const T* xs, int ncol, long long ld, hx_teacher te, double temperature,
-                                                           double scale, const double* __restrict__ weight, T* gs,
-                                                           long long ldg, typename Ty<T>::W* __restrict__ row_loss) {
+constexpr int kScanSlots = 128;  // up to here a slot looks for earlier ones of its position one by one, above in a hash table
+constexpr int kHash = 2048;
+
+static_assert(HX_READOUT_MAX_ROW_BYTES / 2 <= 1 << 20 && HX_READOUT_MAX_K <= 1 << 10, "a position and a slot share 32 bits in the hash table");
+
+size_t distill_extra(int k) { return ((size_t)k * (8 + 8 + 4) + 15) / 16 * 16 + (k > kScanSlots ? kHash * 4 : 0); }
+
+template <typename T, int NT, bool CL>
+__global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == 512 ? 2 : 1)
+    distill_kernel(const T* xs, int nrow, int ncol, long long ld, hx_teacher te, double temperature, double scale,
+                   const double* __restrict__ weight, T* gs, long long ldg, typename Ty<T>::W* __restrict__ row_loss,
+                   int team_bytes, int slice_bytes) {
     using W = typename Ty<T>::W;
-    extern __shared__ unsigned inside[];  // one bit per column: in a slot
-    __shared__ double red[kThreads];
-    __shared__ double sq[HX_READOUT_MAX_K], sx[HX_READOUT_MAX_K];
-    __shared__ int si[HX_READOUT_MAX_K];
-    const size_t row = blockIdx.x;
-    const T* x = xs + row * ld;
+    constexpr int VEC = Ty<T>::VEC;
+    extern __shared__ __align__(16) char smem[];
+    char* mine = smem + (NT == 32 ? (threadIdx.x >> 5) * team_bytes : 0);
+    Team<NT, CL> team(mine);
+    const size_t row = team.row_of_block(team.parts);
+    if (NT == 32 && row >= (size_t)nrow) return;
+    const int t = team.t, k = te.k;
+    const Slice<T> sl((T*)(mine + kRedBytes), xs + row * ld, ncol, team.part, team.parts);
+    double* sq = (double*)(mine + kRedBytes + slice_bytes);  // the slots: value, then probability
+    double* sx = sq + k;                                     // the row's readout there
+    int* si = (int*)(sx + k);                                // position, -1: not used
+    unsigned* hash = (unsigned*)(mine + kRedBytes + slice_bytes + ((size_t)k * 20 + 15) / 16 * 16);
     T* g = gs ? gs + row * ldg : nullptr;
-    const int k = te.k;
     const double w = weight ? weight[row] : 1.0;
     const double inv = 1.0 / temperature;
-    for (int i = threadIdx.x; i < (ncol + 31) / 32; i += kThreads) inside[i] = 0;
-    for (int j = threadIdx.x; j < k; j += kThreads) {
+    if (w != 0.0) sl.template load<NT>(t);
+
+    // the slots
+    if (k > kScanSlots)
+        for (int j = t; j < kHash; j += NT) hash[j] = ~0u;
+    for (int j = t; j < k; j += NT) {
         const int i = te.idx[row * k + j];
         const double v = load_any(te.val, te.dtype, row * k + j);
         si[j] = i >= 0 && i < ncol && v != -INFINITY ? i : -1;
         sq[j] = v;
     }
-    __syncthreads();
-    int used = 0;
-    for (int j = threadIdx.x; j < k; j += kThreads) {
-        bool twice = false;
-        for (int l = 0; l < j; l++) twice |= si[l] == si[j];
-        sx[j] = twice ? 1.0 : 0.0;
-    }
-    __syncthreads();
-    for (int j = threadIdx.x; j < k; j += kThreads) {
-        if (sx[j] != 0.0) si[j] = -1;
-        if (si[j] >= 0) {
-            used = 1;
-            atomicOr(&inside[si[j] >> 5], 1u << (si[j] & 31));
+    team.sync();
+    if (k > kScanSlots) {
+        for (int j = t; j < k; j += NT) {
+            const int i = si[j];
+            if (i < 0) continue;
+            const unsigned both = (unsigned)i << 10 | (unsigned)j;
+            int h = (int)(((unsigned)i * 2654435761u) >> 21);
+            for (int step = 0; step < kHash; step++, h = (h + 1) & (kHash - 1)) {  // at most kHash / 2 places are taken
+                const unsigned o = atomicCAS(&hash[h], ~0u, both);
+                if (o == ~0u) break;
+                if (o >> 10 == (unsigned)i) {
+                    atomicMin(&hash[h], both);
+                    break;
+                }
+            }
         }
+        team.sync();
     }
-    used = block_max(used, (int*)red);
-    W mx = -INFINITY;
-    int bad = 0;
-    if (w != 0.0 && used)
-        for (int i = threadIdx.x; i < ncol; i += kThreads) {
-            const W v = wide(x[i]);
-            if (v > mx) mx = v;
-            bad |= v != v;
+    double tm = -INFINITY;
+    bool used = false;
+    for (int j = t; j < k; j += NT) {
+        const int i = si[j];
+        bool first = i >= 0;
+        if (k > kScanSlots) {
+            if (first) {
+                int h = (int)(((unsigned)i * 2654435761u) >> 21);
+                for (int step = 0; step < kHash && hash[h] >> 10 != (unsigned)i; step++) h = (h + 1) & (kHash - 1);
+                first = (hash[h] & 1023) == (unsigned)j;
+            }
+        } else {
+            for (int l = 0; l < j; l++) first &= si[l] != i;
         }
-    mx = (W)block_max((double)mx, red);
-    bad = block_max(bad, (int*)red);
-    if (w == 0.0 || !used || (mx == -INFINITY && !bad)) {
-        if (threadIdx.x == 0) row_loss[row] = 0;
-        if (g)
-            for (int i = threadIdx.x; i < ncol; i += kThreads) put(&g[i], (W)0);
+        sx[j] = first ? 1.0 : 0.0;
+        used |= first;
+        if (first) tm = sq[j] > tm || sq[j] != sq[j] ? sq[j] : tm;
+    }
+    used = team.any(used) && w != 0.0;
+    if (used) {
+        for (int j = t; j < k; j += NT)
+            if (sx[j] == 0.0) si[j] = -1;
+    } else {  // the same in every block of a cluster
+        if (t == 0 && team.part == 0) row_loss[row] = 0;
+        sl.wait();
+        if (g) sl.template store<NT>(t, g, [](int) {
+            Vec<T> z;
+#pragma unroll
+            for (int u = 0; u < VEC; u++) z.e[u] = narrow<T>((W)0);
+            return z;
+        });
         return;
     }
-    if (bad) mx = NAN;
-    const W winv = (W)inv;
-    W s_in = 0, s_out = 0;
-    for (int i = threadIdx.x; i < ncol; i += kThreads) {
-        const W e = exp((wide(x[i]) - mx) * winv);
-        if (inside[i >> 5] >> (i & 31) & 1)
-            s_in += e;
-        else
-            s_out += e;
-    }
-    const double sum_in = (double)block_sum(s_in, (W*)red), sum_out = (double)block_sum(s_out, (W*)red);
-    const double total = sum_in + sum_out, log_total = log(total);
-    // the teacher's q in the slots
     double norm;
     if (te.lse) {
         norm = load_any(te.lse, te.dtype == HX_DT_F64 ? HX_DT_F64 : HX_DT_F32, row);
     } else {
-        double tm = -INFINITY;
-        for (int j = threadIdx.x; j < k; j += kThreads)
-            if (si[j] >= 0) tm = sq[j] > tm || sq[j] != sq[j] ? sq[j] : tm;
-        tm = block_reduce(tm, red, [](double a, double b) { return a > b || a != a ? a : b; });
+        tm = team.template reduce<false>(tm, [](double a, double b) { return a > b || a != a ? a : b; });
         double ts = 0;
-        for (int j = threadIdx.x; j < k; j += kThreads)
+        for (int j = t; j < k; j += NT)
             if (si[j] >= 0) ts += exp((sq[j] - tm) * inv);
-        ts = block_sum(ts, red);
+        ts = team.template reduce<false>(ts, [](double a, double b) { return a + b; });
         norm = tm * inv + log(ts);
     }
-    double qs = 0, loss = 0;
-    for (int j = threadIdx.x; j < k; j += kThreads) {
+    struct Pair {
+        double a, b;
+    } qa{0, 0};  // sum of q, sum of q log q
+    for (int j = t; j < k; j += NT) {
         if (si[j] < 0) continue;
         const double lq = sq[j] * inv - norm, q = exp(lq);
-        const double lp = ((double)wide(x[si[j]]) - (double)mx) * inv - log_total;
-        sx[j] = lp;
         sq[j] = q;
-        qs += q;
-        loss += q == 0.0 ? 0.0 : q * (lq - lp);
+        qa.a += q;
+        qa.b += q == 0.0 ? 0.0 : q * lq;
     }
-    qs = block_sum(qs, red);
-    loss = block_sum(loss, red);
-    double qr = te.lse ? (qs == qs ? fmax(0.0, 1.0 - qs) : qs) : 0.0;
-    const double pr = sum_out / total;
-    if (qr > 0.0 && sum_out > 0.0)
+    qa = team.template reduce<false>(qa, [](Pair x, Pair y) { return Pair{x.a + y.a, x.b + y.b}; });
+
+    // the row is here: lift the slots' readouts out of it
+    sl.wait();
+    team.sync();
+    W mx = -INFINITY;
+    for (int j = t; j < k; j += NT) {
+        const int i = si[j] - sl.first;
+        if (si[j] >= 0 && i >= 0 && i < sl.n) {
+            const W v = wide(sl.e[sl.phase + i]);
+            sx[j] = (double)v;
+            mx = max_num(mx, v);
+            sl.e[sl.phase + i] = narrow<T>((W)-INFINITY);
+        }
+    }
+    team.sync();
+    for (int v = t; v < sl.nv; v += NT) {
+        const Vec<T> x = sl.get(v);
+#pragma unroll
+        for (int u = 0; u < VEC; u++) mx = max_num(mx, wide(x.e[u]));
+    }
+    mx = team.template reduce<true>(mx, [](W a, W b) { return max_num(a, b); });
+    const W m0 = mx == -INFINITY ? (W)0 : mx;
+    const auto ex = scaler((W)0, temperature);
+    struct Sums {
+        double out, in, qz;
+    } s{0, 0, 0};
+    {
+        W part[2] = {0, 0};
+        for (int v = t; v < sl.nv; v += NT) {
+            Vec<T> x = sl.get(v);
+#pragma unroll
+            for (int u = 0; u < VEC; u++) {
+                const W e = ex(wide(x.e[u]) - m0);
+                part[u & 1] += e;
+                if constexpr (sizeof(T) == sizeof(W)) x.e[u] = e;
+            }
+            if constexpr (sizeof(T) == sizeof(W)) sl.set(v, x);
+        }
+        s.out = (double)part[0] + (double)part[1];
+    }
+    for (int j = t; j < k; j += NT) {
+        const int i = si[j] - sl.first;
+        if (si[j] >= 0 && i >= 0 && i < sl.n) {
+            const double z = (sx[j] - (double)m0) * inv;
+            s.in += exp(z);
+            s.qz += sq[j] == 0.0 ? 0.0 : sq[j] * z;
+        }
+    }
+    s = team.template reduce<true>(s, [](Sums a, Sums b) { return Sums{a.out + b.out, a.in + b.in, a.qz + b.qz}; });
+    const double total = s.in + s.out;
+    const bool empty = mx == -INFINITY && total == 0.0;  // NaN in the row makes the sums NaN
+    double qr = te.lse ? (qa.a == qa.a ? fmax(0.0, 1.0 - qa.a) : qa.a) : 0.0;
+    const double pr = s.out / total;
+    double loss = qa.b - s.qz + qa.a * log(total);
+    if (qr > 0.0 && s.out > 0.0)
         loss += qr * (log(qr) - log(pr));
-    else if (qr == qr)
+    else if (qr == qr && s.out == s.out)
         qr = 0.0;
-    if (threadIdx.x == 0) row_loss[row] = (W)(temperature * temperature * loss);
-    if (!g) return;
-    const double c = scale * w * temperature, mass = te.lse ? qs + qr : 1.0;
-    const W a_in = (W)(c * mass / total), a_out = qr == 0.0 ? a_in : (W)(c * (mass - qr / pr) / total);
-    __syncthreads();
-    for (int i = threadIdx.x; i < ncol; i += kThreads) {
-        const W e = exp((wide(x[i]) - mx) * winv);
-        if (!(inside[i >> 5] >> (i & 31) & 1)) put(&g[i], a_out * e);
+    if (t == 0 && team.part == 0) row_loss[row] = empty ? (W)0 : (W)(temperature * temperature * loss);
+    if (g) {
+        const double c = empty ? 0.0 : scale * w * temperature;
+        const double mass = te.lse || qa.a != qa.a ? qa.a + qr : 1.0;
+        const W a_out = empty ? (W)0 : (W)(c * (qr == 0.0 ? mass : mass - qr / pr) / total);
+        sl.template store<NT>(t, g, [&](int v) {
+            Vec<T> x = sl.get(v);
+#pragma unroll
+            for (int u = 0; u < VEC; u++) {
+                if constexpr (sizeof(T) == sizeof(W))
+                    x.e[u] = x.e[u] * a_out;
+                else
+                    x.e[u] = narrow<T>(ex(wide(x.e[u]) - m0) * a_out);
+            }
+            return x;
+        });
+        team.sync();
+        for (int j = t; j < k; j += NT) {
+            const int i = si[j] - sl.first;
+            if (si[j] >= 0 && i >= 0 && i < sl.n) {
+                const double p = exp((sx[j] - (double)m0) * inv) / total;
+                g[si[j]] = narrow<T>(empty ? (W)0 : (W)(c * (mass * p - sq[j])));
+            }
+        }
     }
-    for (int j = threadIdx.x; j < k; j += kThreads)
-        if (si[j] >= 0) put(&g[si[j]], (W)(c * (mass * exp(sx[j]) - sq[j])));
+    if constexpr (CL) team.sync_all();  // a block stays while others may read its partials
 }
 
 template <typename W>
@@ -566,6 +622,57 @@ struct OnDevice {
     }
 };
 
+// How a call's rows are dealt to threads.
+struct Deal {
+    int nt, parts;
+    size_t slice, team;  // bytes of shared memory: of a slice, of a team's part
+};
+constexpr size_t kSmemBlock = 227 * 1024;
+
+// Warps take short rows, blocks of 128 and 512 threads longer ones.  A row
+// that no block can hold is shared by a cluster of blocks, and one of few rows
+// too, so that the card is not left idle.
+template <typename T>
+Deal deal(const hx_readout* r, size_t extra, int sms) {
+    Deal d{};
+    d.parts = 1;
+    if (r->ncol <= 512 && extra <= 6144) {
+        d.nt = 32;
+    } else {
+        while (d.parts < 8 && kRedBytes + Slice<T>::bytes(r->ncol, d.parts) + extra > kSmemBlock) d.parts *= 2;
+        while (d.parts < 8 && (long long)r->nrow * d.parts * 2 <= sms && r->ncol / d.parts >= 4096) d.parts *= 2;
+        d.nt = d.parts == 1 && r->ncol <= 2048 ? 128 : 512;
+    }
+    d.slice = Slice<T>::bytes(r->ncol, d.parts);
+    d.team = kRedBytes + d.slice + (extra + 15) / 16 * 16;
+    return d;
+}
+
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), const Deal& d, int nrow, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t c{};
+    c.dynamicSmemBytes = d.nt == 32 ? d.team * kWarpRows : d.team;
+    if (c.dynamicSmemBytes > 48 * 1024)
+        if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)c.dynamicSmemBytes)) return e;
+    c.gridDim = dim3(d.nt == 32 ? (unsigned)((nrow + kWarpRows - 1) / kWarpRows) : (unsigned)nrow * d.parts);
+    c.blockDim = dim3(d.nt == 32 ? 32 * kWarpRows : d.nt);
+    c.stream = st;
+    cudaLaunchAttribute a;
+    a.id = cudaLaunchAttributeClusterDimension;
+    a.val.clusterDim.x = d.parts;
+    a.val.clusterDim.y = a.val.clusterDim.z = 1;
+    if (d.parts > 1) {
+        c.attrs = &a;
+        c.numAttrs = 1;
+    }
+    return cudaLaunchKernelEx(&c, kernel, P(args)...);
+}
+
+int sm_count(int device) {
+    int n = 0;
+    return cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) == cudaSuccess ? n : 1;
+}
+
 template <typename F>
 int by_type(int dtype, F f) {
     switch (dtype) {
@@ -627,12 +734,14 @@ int hx_distill_loss_grad_dev(hx_ctx* ctx, const hx_readout* rows, const hx_teach
     return by_type(rows->dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         using W = typename Ty<T>::W;
-        const size_t smem = (size_t)(rows->ncol + 31) / 32 * 4;
-        HXC(cudaFuncSetAttribute(distill_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         if (rows->nrow > 0) {
-            distill_kernel<T><<<rows->nrow, kThreads, smem, ctx->st>>>((const T*)rows->x, rows->ncol, rows->ld, *teacher, temperature,
-                                                                       scale, row_weight_dev, (T*)grad_dev, ld_grad, (W*)row_loss_dev);
-            HXC(cudaGetLastError());
+            const Deal d = deal<T>(rows, distill_extra(teacher->k), sm_count(ctx->device));
+            auto go = [&](auto* kernel) {
+                return launch(kernel, d, rows->nrow, ctx->st, (const T*)rows->x, rows->nrow, rows->ncol, rows->ld, *teacher, temperature,
+                              scale, row_weight_dev, (T*)grad_dev, ld_grad, (W*)row_loss_dev, (int)d.team, (int)d.slice);
+            };
+            HXC(d.nt == 32 ? go(distill_kernel<T, 32, false>) : d.parts > 1 ? go(distill_kernel<T, 512, true>)
+                : d.nt == 128 ? go(distill_kernel<T, 128, false>) : go(distill_kernel<T, 512, false>));
         }
         loss_kernel<W><<<1, kThreads, 0, ctx->st>>>((const W*)row_loss_dev, row_weight_dev, rows->nrow, scale, (W*)loss_dev);
         HXC(cudaGetLastError());

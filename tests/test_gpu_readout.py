@@ -31,7 +31,7 @@ pytestmark = pytest.mark.gpu
 
 DT = {"f64": torch.float64, "f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 HALF = {"f64": 2.0**-53, "f32": 2.0**-24, "f16": 2.0**-11, "bf16": 2.0**-8}
-TINY = {"f64": 0.0, "f32": 2.0**-149, "f16": 2.0**-25, "bf16": 2.0**-134}  # half a subnormal step (fp32: flushed results too)
+TINY = {"f64": 0.0, "f32": 2.0**-126, "f16": 2.0**-25, "bf16": 2.0**-126}  # fp32 exponentials below 2^-126 are 0; fp16: half a subnormal step
 STAT = {"f64": torch.float64, "f32": torch.float32, "f16": torch.float32, "bf16": torch.float32}
 
 
