@@ -4,9 +4,11 @@
 // One thread block per row; the row is read from global memory once per pass.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdio>
+#include <cstring>
 #include <string>
 #include <type_traits>
 
@@ -19,6 +21,7 @@ namespace {
 using namespace hxr;
 
 constexpr int kThreads = 256;
+constexpr int kBlock = 256;  // threads of a block that has a row, or a slice of one, to itself (short rows: 128)
 
 __device__ __forceinline__ void put(double* p, double v) { *p = v; }
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
@@ -204,59 +207,91 @@ __global__ void __launch_bounds__(kThreads) top_kernel(const T* __restrict__ xs,
 
 // ---------------------------------------------------------------- distillation
 //
-// One pass over memory: the row waits in shared memory while its maximum, the
-// sum of its exponentials and then the gradient are taken.  The slots' readouts
-// are lifted out of the row first (-inf stands in their places), so that the
-// sum over the rest is a sum of its own and not a difference.  The teacher's
-// side is worked out while the row is on its way.
+// One pass over memory, and as few instructions as it takes: the row waits in
+// shared memory, is replaced there by its exponentials, these by the gradient,
+// and leaves in bulk copies.  Every warp has a run of the row's vectors of its
+// own, for which it waits, and asks for that run of the team's next row when
+// the bulk copy has read the last.  The warps of a row meet twice: before it,
+// when the teacher's side is ready, and for the sum.
+//
+// The exponentials are taken relative to the readout in the first slot, which
+// the teacher holds for likely, not to the row's largest: only where the sum
+// then shows that some other readout is far above it (e^28 times in fp32,
+// e^346 in fp64), or NaN, is the row read again and its largest found.
+//
+// The slots' readouts are lifted out of the row before the sum (-inf stands in
+// their places), so that the sum over the rest is a sum of its own and not a
+// difference.  The teacher's side of the next row is worked out meanwhile: in
+// a block of many warps by a helper, which has no run, so that its chain of
+// dependent exponentials and reductions is waited for by nobody.
 
-constexpr int kScanSlots = 128;  // up to here a slot looks for earlier ones of its position one by one, above in a hash table
-constexpr int kHash = 2048;
+constexpr int kFewSlots = 128;  // up to here the next row's slots are worked out into lists of their own
 
+__host__ __device__ constexpr int slot_list(int k) { return (k + 3) / 4 * 4; }
+__host__ __device__ constexpr int hash_bits(int k) {  // a table at most half full
+    int b = 5;
+    while ((1 << b) < 2 * k) b++;
+    return b;
+}
 static_assert(HX_READOUT_MAX_ROW_BYTES / 2 <= 1 << 20 && HX_READOUT_MAX_K <= 1 << 10, "a position and a slot share 32 bits in the hash table");
+size_t distill_extra(int k) { return (size_t)slot_list(k) * 20 * (k <= kFewSlots ? 2 : 1) + ((size_t)4 << hash_bits(k)); }
 
-size_t distill_extra(int k) { return ((size_t)k * (8 + 8 + 4) + 15) / 16 * 16 + (k > kScanSlots ? kHash * 4 : 0); }
-
-template <typename T, int NT, bool CL>
-__global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == 512 ? 2 : 1)
-    distill_kernel(const T* xs, int nrow, int ncol, long long ld, hx_teacher te, double temperature, double scale,
-                   const double* __restrict__ weight, T* gs, long long ldg, typename Ty<T>::W* __restrict__ row_loss,
-                   int team_bytes, int slice_bytes) {
-    using W = typename Ty<T>::W;
-    constexpr int VEC = Ty<T>::VEC;
-    extern __shared__ __align__(16) char smem[];
-    char* mine = smem + (NT == 32 ? (threadIdx.x >> 5) * team_bytes : 0);
-    Team<NT, CL> team(mine);
-    const size_t row = team.row_of_block(team.parts);
-    if (NT == 32 && row >= (size_t)nrow) return;
-    const int t = team.t, k = te.k;
-    const Slice<T> sl((T*)(mine + kRedBytes), xs + row * ld, ncol, team.part, team.parts);
-    double* sq = (double*)(mine + kRedBytes + slice_bytes);  // the slots: value, then probability
-    double* sx = sq + k;                                     // the row's readout there
-    int* si = (int*)(sx + k);                                // position, -1: not used
-    unsigned* hash = (unsigned*)(mine + kRedBytes + slice_bytes + ((size_t)k * 20 + 15) / 16 * 16);
-    T* g = gs ? gs + row * ldg : nullptr;
-    const double w = weight ? weight[row] : 1.0;
-    const double inv = 1.0 / temperature;
-    if (w != 0.0) sl.template load<NT>(t);
-
-    // the slots
-    if (k > kScanSlots)
-        for (int j = t; j < kHash; j += NT) hash[j] = ~0u;
-    for (int j = t; j < k; j += NT) {
-        const int i = te.idx[row * k + j];
-        const double v = load_any(te.val, te.dtype, row * k + j);
-        si[j] = i >= 0 && i < ncol && v != -INFINITY ? i : -1;
-        sq[j] = v;
+// The slots of a row, in shared memory, and the warp that works on them
+// (lane l has slots l, l + 32, ...).
+struct Slots {
+    double* q;  // value, then probability
+    double* x;  // exponential of the row's readout there
+    int* at;    // position, -1: not used
+    double* notes;  // [0] log-sum-exp of the record, [1] sum of q, [2] sum of q log q, [3] 1: a slot is used, [4] a readout there
+    int lane;
+    __device__ Slots(char* lists, double* all_notes, int k, int set, int thread) : lane(thread & 31) {
+        q = (double*)(lists + (k <= kFewSlots ? set * slot_list(k) * 20 : 0));
+        x = q + slot_list(k);
+        at = (int*)(x + slot_list(k));
+        notes = all_notes + set * 8;
     }
-    team.sync();
-    if (k > kScanSlots) {
-        for (int j = t; j < k; j += NT) {
-            const int i = si[j];
-            if (i < 0) continue;
+    static __device__ __forceinline__ double sum(double v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+        return v;
+    }
+    // Starts the copy of a row's record; narrow values are widened at once.
+    __device__ __forceinline__ void load(const hx_teacher& te, size_t row) const {
+        const int k = te.k;
+        for (int j = lane; j < k; j += 32) {
+            copy4(at + j, te.idx + row * k + j);
+            if (te.dtype == HX_DT_F64)
+                copy8(q + j, (const double*)te.val + row * k + j);
+            else if (te.dtype == HX_DT_F32)
+                copy4(q + j, (const float*)te.val + row * k + j);
+            else
+                q[j] = load_any(te.val, te.dtype, row * k + j);
+        }
+        if (te.lse && lane == 0) {
+            if (te.dtype == HX_DT_F64)
+                copy8(notes, (const double*)te.lse + row);
+            else
+                copy4(notes, (const float*)te.lse + row);
+        }
+    }
+    // Positions, probabilities and sums from the copied record; GROUPS of later copies may be on their way.
+    template <int GROUPS, typename T>
+    __device__ __forceinline__ void work_out(const hx_teacher& te, const T* row, int ncol, double inv, unsigned* hash) const {
+        const int k = te.k, bits = hash_bits(k), most = 1 << bits;
+        wait_copies<GROUPS>();
+        if (k > 32)
+            for (int h = lane; h < most; h += 32) hash[h] = ~0u;
+        __syncwarp();
+        for (int j = lane; j < k; j += 32) {
+            const double v = te.dtype == HX_DT_F32 ? (double)*(const float*)(q + j) : q[j];
+            int i = at[j];
+            q[j] = v;
+            if (i < 0 || i >= ncol || v == -INFINITY) i = -1;
+            at[j] = i;
+            if (k <= 32 || i < 0) continue;
             const unsigned both = (unsigned)i << 10 | (unsigned)j;
-            int h = (int)(((unsigned)i * 2654435761u) >> 21);
-            for (int step = 0; step < kHash; step++, h = (h + 1) & (kHash - 1)) {  // at most kHash / 2 places are taken
+            unsigned h = ((unsigned)i * 2654435761u) >> (32 - bits);
+            for (int step = 0; step < most; step++, h = (h + 1) & (most - 1)) {
                 const unsigned o = atomicCAS(&hash[h], ~0u, both);
                 if (o == ~0u) break;
                 if (o >> 10 == (unsigned)i) {
@@ -265,145 +300,255 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == 512 ? 2 
                 }
             }
         }
-        team.sync();
-    }
-    double tm = -INFINITY;
-    bool used = false;
-    for (int j = t; j < k; j += NT) {
-        const int i = si[j];
-        bool first = i >= 0;
-        if (k > kScanSlots) {
-            if (first) {
-                int h = (int)(((unsigned)i * 2654435761u) >> 21);
-                for (int step = 0; step < kHash && hash[h] >> 10 != (unsigned)i; step++) h = (h + 1) & (kHash - 1);
-                first = (hash[h] & 1023) == (unsigned)j;
+        __syncwarp();
+        // a position that an earlier slot has is dropped
+        double tm = -INFINITY;
+        bool used = false;
+        if (k <= 32) {
+            const int i = lane < k ? at[lane] : -1;
+            const unsigned same = __match_any_sync(~0u, i);
+            if (i >= 0 && __ffs(same) - 1 == lane) {
+                used = true;
+                tm = larger(tm, q[lane]);
+            } else if (lane < k) {
+                at[lane] = -1;
             }
         } else {
-            for (int l = 0; l < j; l++) first &= si[l] != i;
+            for (int j = lane; j < k; j += 32) {
+                const int i = at[j];
+                if (i < 0) continue;
+                unsigned h = ((unsigned)i * 2654435761u) >> (32 - bits);
+                for (int step = 0; step < most && hash[h] >> 10 != (unsigned)i; step++) h = (h + 1) & (most - 1);
+                if ((hash[h] & 1023) == (unsigned)j) {
+                    used = true;
+                    tm = larger(tm, q[j]);
+                } else {
+                    at[j] = -1;
+                }
+            }
         }
-        sx[j] = first ? 1.0 : 0.0;
-        used |= first;
-        if (first) tm = sq[j] > tm || sq[j] != sq[j] ? sq[j] : tm;
-    }
-    used = team.any(used) && w != 0.0;
-    if (used) {
-        for (int j = t; j < k; j += NT)
-            if (sx[j] == 0.0) si[j] = -1;
-    } else {  // the same in every block of a cluster
-        if (t == 0 && team.part == 0) row_loss[row] = 0;
-        sl.wait();
-        if (g) sl.template store<NT>(t, g, [](int) {
-            Vec<T> z;
+        __syncwarp();
+        const unsigned lanes = __ballot_sync(~0u, used);
+        T ref = narrow<T>((typename Ty<T>::W)0);
+        if (lanes) {
+            int j = __ffs(lanes) - 1;
+            while (at[j] < 0) j += 32;  // that lane's first slot in use
+            ref = row[at[j]];
+        }
+        double shift;
+        if (te.lse) {
+            shift = te.dtype == HX_DT_F64 ? notes[0] : (double)*(const float*)notes;
+            tm = 0;
+        } else {
 #pragma unroll
-            for (int u = 0; u < VEC; u++) z.e[u] = narrow<T>((W)0);
-            return z;
-        });
-        return;
+            for (int o = 16; o > 0; o >>= 1) tm = larger(tm, __shfl_xor_sync(~0u, tm, o));
+            shift = 0;
+        }
+        double s = 0, qv = 0;
+        for (int j = lane; j < k; j += 32) {
+            if (at[j] < 0) continue;
+            const double lq = (q[j] - tm) * inv - shift, e = exp(lq);
+            q[j] = e;
+            s += e;
+            qv += e == 0.0 ? 0.0 : e * lq;
+        }
+        s = sum(s);
+        qv = sum(qv);
+        if (!te.lse) {  // over the slots alone: divide by their sum
+            const double f = 1.0 / s;
+            for (int j = lane; j < k; j += 32)
+                if (at[j] >= 0) q[j] *= f;
+            qv = qv * f - log(s);
+            s = s == s ? 1.0 : s;
+        }
+        __syncwarp();
+        if (lane == 0) {
+            notes[1] = s;
+            notes[2] = qv;
+            notes[3] = lanes ? 1.0 : 0.0;
+            notes[4] = (double)wide(ref);
+        }
     }
-    double norm;
-    if (te.lse) {
-        norm = load_any(te.lse, te.dtype == HX_DT_F64 ? HX_DT_F64 : HX_DT_F32, row);
-    } else {
-        tm = team.template reduce<false>(tm, [](double a, double b) { return a > b || a != a ? a : b; });
-        double ts = 0;
-        for (int j = t; j < k; j += NT)
-            if (si[j] >= 0) ts += exp((sq[j] - tm) * inv);
-        ts = team.template reduce<false>(ts, [](double a, double b) { return a + b; });
-        norm = tm * inv + log(ts);
+    // f(j, cell) for the slots whose readouts are in vectors v0 .. v1-1 of the slice.
+    template <typename T, typename F>
+    __device__ __forceinline__ void each(const Slice<T>& sl, int k, int v0, int v1, F f) const {
+        const int a = max(v0 * Ty<T>::VEC, sl.phase), n = min(v1 * Ty<T>::VEC, sl.phase + sl.n) - a, shift = sl.phase - sl.first;
+        for (int j = lane; j < k; j += 32) {
+            const int p = at[j];
+            if (p >= 0 && (unsigned)(p + shift - a) < (unsigned)max(n, 0)) f(j, sl.e + (p + shift));
+        }
     }
-    struct Pair {
-        double a, b;
-    } qa{0, 0};  // sum of q, sum of q log q
-    for (int j = t; j < k; j += NT) {
-        if (si[j] < 0) continue;
-        const double lq = sq[j] * inv - norm, q = exp(lq);
-        sq[j] = q;
-        qa.a += q;
-        qa.b += q == 0.0 ? 0.0 : q * lq;
-    }
-    qa = team.template reduce<false>(qa, [](Pair x, Pair y) { return Pair{x.a + y.a, x.b + y.b}; });
+};
 
-    // the row is here: lift the slots' readouts out of it
-    sl.wait();
-    team.sync();
-    W mx = -INFINITY;
-    for (int j = t; j < k; j += NT) {
-        const int i = si[j] - sl.first;
-        if (si[j] >= 0 && i >= 0 && i < sl.n) {
-            const W v = wide(sl.e[sl.phase + i]);
-            sx[j] = (double)v;
-            mx = max_num(mx, v);
-            sl.e[sl.phase + i] = narrow<T>((W)-INFINITY);
-        }
+template <typename T, int NT, bool CL>
+__global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT + 32, NT == kBlock ? 2 : 6)
+    distill_kernel(const T* xs, int nrow, int ncol, long long ld, hx_teacher te, Heat heat, double scale,
+                   const double* __restrict__ weight, T* gs, long long ldg, typename Ty<T>::W* __restrict__ row_loss,
+                   int team_bytes, int slice_bytes) {
+    using W = typename Ty<T>::W;
+    constexpr int VEC = Ty<T>::VEC;
+    constexpr bool ONE = NT == 32;  // one warp does it all
+    constexpr int UNROLL = VEC == 8 ? 1 : 2;
+    extern __shared__ __align__(16) char smem[];
+    char* const mine = smem + (ONE ? (threadIdx.x >> 5) * team_bytes : 0);
+    Team<NT, CL, !ONE> team(mine);
+    const int t = team.t, k = te.k;
+    const bool few = k <= kFewSlots;
+    const bool helper = ONE || t >= NT, worker = ONE || t < NT;
+    T* const row_mem = (T*)(mine + kRedBytes);
+    char* const lists = mine + kRedBytes + slice_bytes;
+    unsigned* const hash = (unsigned*)(lists + slot_list(k) * 20 * (few ? 2 : 1));
+    const long long step = team.row_step();
+    long long row = team.first_row();
+    if (row >= nrow) return;  // a whole team
+    double w = weight ? weight[row] : 1.0;
+    int set = 0;
+    const int lane = t & 31, warp = ONE ? 0 : t >> 5;
+    constexpr int NW = NT / 32;
+    const auto ask = [&](const Slice<T>& s) {  // for this warp's run
+        s.load(s.template run<NW>(warp), s.template run<NW>(warp + 1), lane);
+    };
+    if (w != 0.0) {
+        const Slots slots(lists, team.notes(), k, 0, t);
+        const T* const x = xs + row * ld;
+        if (helper) slots.load(te, row);
+        if (ONE) commit_copies();
+        if (worker) ask(Slice<T>(row_mem, x, ncol, team.part, team.parts));
+        if (ONE) commit_copies();
+        if (helper) slots.template work_out<ONE ? 1 : 0>(te, x, ncol, heat.inv, hash);
     }
-    team.sync();
-    for (int v = t; v < sl.nv; v += NT) {
-        const Vec<T> x = sl.get(v);
+    for (;;) {
+        const Slice<T> sl(row_mem, xs + row * ld, ncol, team.part, team.parts);
+        const int v0 = sl.template run<NW>(warp), v1 = sl.template run<NW>(warp + 1);
+        T* const g = gs ? gs + row * ldg : nullptr;
+        const long long next = row + step;
+        const double wn = next < nrow ? (weight ? weight[next] : 1.0) : 0.0;
+        const Slots slots(lists, team.notes(), k, set, t), ahead(lists, team.notes(), k, set ^ 1, t);
+        bool live = w != 0.0;
+        if (worker) wait_copies();
+        team.sync_block();  // the slots are ready, and those of the row before are free
+        live = live && slots.notes[3] != 0.0;
+        // the next row's record, before the row's own traffic
+        if (helper && few && wn != 0.0) ahead.load(te, next);
+        if (ONE) commit_copies();
+        if (live) {
+            struct Sums {
+                double out, in, qz;
+            } s;
+            W m = (W)slots.notes[4];
+            bool odd = false, empty = false;  // NaN or +inf in the row; no readout is open
+            for (bool sure = false;; sure = true) {
+                if (sure) {  // the row's largest readout
+                    struct Top {
+                        W mx;
+                        int odd;
+                    } top{(W)-INFINITY, 0};
+                    if (worker) {
+                        __syncwarp();
+                        ask(sl);
+                        wait_copies();
+                        for (int v = v0 + lane; v < v1; v += 32) {
+                            const Vec<T> x = sl.get(v);
 #pragma unroll
-        for (int u = 0; u < VEC; u++) mx = max_num(mx, wide(x.e[u]));
-    }
-    mx = team.template reduce<true>(mx, [](W a, W b) { return max_num(a, b); });
-    const W m0 = mx == -INFINITY ? (W)0 : mx;
-    const auto ex = scaler((W)0, temperature);
-    struct Sums {
-        double out, in, qz;
-    } s{0, 0, 0};
-    {
-        W part[2] = {0, 0};
-        for (int v = t; v < sl.nv; v += NT) {
-            Vec<T> x = sl.get(v);
+                            for (int u = 0; u < VEC; u++) {
+                                const W y = wide(x.e[u]);
+                                top.mx = larger(top.mx, y);
+                                top.odd |= !(y < (W)INFINITY);
+                            }
+                        }
+                        __syncwarp();
+                    }
+                    const auto op = [](Top a, Top b) { return Top{larger(a.mx, b.mx), a.odd | b.odd}; };
+                    top = team.across(team.reduce(top, op), op);
+                    odd = top.odd;
+                    empty = top.mx == (W)-INFINITY && !odd;
+                    m = odd || empty ? (W)0 : top.mx;
+                }
+                const auto ex = scaler(m, heat, team.table());
+                s = Sums{0, 0, 0};
+                if (worker) {
+                    slots.each(sl, k, v0, v1, [&](int j, T* cell) {
+                        const double z = ex.z((double)wide(*cell)), e = exp(z), q = slots.q[j];
+                        *cell = narrow<T>((W)-INFINITY);
+                        slots.x[j] = e;
+                        s.in += e;
+                        s.qz += q == 0.0 ? 0.0 : q * z;
+                    });
+                    __syncwarp();
+                    W part[2] = {0, 0};
+#pragma unroll UNROLL
+                    for (int v = v0 + lane; v < v1; v += 32) {
+                        Vec<T> x = sl.get(v);
 #pragma unroll
-            for (int u = 0; u < VEC; u++) {
-                const W e = ex(wide(x.e[u]) - m0);
-                part[u & 1] += e;
-                if constexpr (sizeof(T) == sizeof(W)) x.e[u] = e;
+                        for (int u = 0; u < VEC; u++) {
+                            const W e = ex(wide(x.e[u]));
+                            part[u & 1] += e;
+                            if constexpr (sizeof(T) == sizeof(W)) x.e[u] = e;
+                        }
+                        if constexpr (sizeof(T) == sizeof(W)) sl.set(v, x);
+                    }
+                    s.out = (double)part[0] + (double)part[1];
+                }
+                const auto op = [](Sums a, Sums b) { return Sums{a.out + b.out, a.in + b.in, a.qz + b.qz}; };
+                s = team.across(team.reduce(s, op), op);
+                if (sure || (s.in + s.out <= decltype(ex)::most && s.in + s.out > 0.0)) break;
             }
-            if constexpr (sizeof(T) == sizeof(W)) sl.set(v, x);
-        }
-        s.out = (double)part[0] + (double)part[1];
-    }
-    for (int j = t; j < k; j += NT) {
-        const int i = si[j] - sl.first;
-        if (si[j] >= 0 && i >= 0 && i < sl.n) {
-            const double z = (sx[j] - (double)m0) * inv;
-            s.in += exp(z);
-            s.qz += sq[j] == 0.0 ? 0.0 : sq[j] * z;
-        }
-    }
-    s = team.template reduce<true>(s, [](Sums a, Sums b) { return Sums{a.out + b.out, a.in + b.in, a.qz + b.qz}; });
-    const double total = s.in + s.out;
-    const bool empty = mx == -INFINITY && total == 0.0;  // NaN in the row makes the sums NaN
-    double qr = te.lse ? (qa.a == qa.a ? fmax(0.0, 1.0 - qa.a) : qa.a) : 0.0;
-    const double pr = s.out / total;
-    double loss = qa.b - s.qz + qa.a * log(total);
-    if (qr > 0.0 && s.out > 0.0)
-        loss += qr * (log(qr) - log(pr));
-    else if (qr == qr && s.out == s.out)
-        qr = 0.0;
-    if (t == 0 && team.part == 0) row_loss[row] = empty ? (W)0 : (W)(temperature * temperature * loss);
-    if (g) {
-        const double c = empty ? 0.0 : scale * w * temperature;
-        const double mass = te.lse || qa.a != qa.a ? qa.a + qr : 1.0;
-        const W a_out = empty ? (W)0 : (W)(c * (qr == 0.0 ? mass : mass - qr / pr) / total);
-        sl.template store<NT>(t, g, [&](int v) {
-            Vec<T> x = sl.get(v);
+            const double sum_q = slots.notes[1], sum_qlq = slots.notes[2];
+            const double total = odd ? (double)NAN : s.in + s.out;
+            double qr = te.lse ? (sum_q == sum_q ? larger(0.0, 1.0 - sum_q) : sum_q) : 0.0;
+            if (!(qr > 0.0 && s.out > 0.0) && qr == qr && s.out == s.out) qr = 0.0;
+            if (worker && g) {
+                const double one_over = 1.0 / total, mass = sum_q + qr, c = empty ? 0.0 : scale * w * heat.t;
+                double a = c * mass * one_over;
+                const double a_in = empty ? 0.0 : a;
+                if (qr != 0.0) a -= c * qr / s.out;
+                const W a_out = empty ? (W)0 : (W)a;
+                const auto ex = scaler(m, heat, team.table());
+#pragma unroll UNROLL
+                for (int v = v0 + lane; v < v1; v += 32) {
+                    Vec<T> x = sl.get(v);
 #pragma unroll
-            for (int u = 0; u < VEC; u++) {
-                if constexpr (sizeof(T) == sizeof(W))
-                    x.e[u] = x.e[u] * a_out;
-                else
-                    x.e[u] = narrow<T>(ex(wide(x.e[u]) - m0) * a_out);
+                    for (int u = 0; u < VEC; u++) {
+                        if constexpr (sizeof(T) == sizeof(W))
+                            x.e[u] = x.e[u] * a_out;
+                        else
+                            x.e[u] = narrow<T>(ex(wide(x.e[u])) * a_out);
+                    }
+                    sl.set(v, x);
+                }
+                __syncwarp();
+                slots.each(sl, k, v0, v1, [&](int j, T* cell) { *cell = narrow<T>((W)(a_in * slots.x[j] - c * slots.q[j])); });
             }
-            return x;
-        });
-        team.sync();
-        for (int j = t; j < k; j += NT) {
-            const int i = si[j] - sl.first;
-            if (si[j] >= 0 && i >= 0 && i < sl.n) {
-                const double p = exp((sx[j] - (double)m0) * inv) / total;
-                g[si[j]] = narrow<T>(empty ? (W)0 : (W)(c * (mass * p - sq[j])));
+            if (helper && lane == 0 && team.part == 0) {
+                double loss = sum_qlq - s.qz + sum_q * log(total);
+                if (qr != 0.0) loss += qr * log(qr * total / s.out);
+                row_loss[row] = empty ? (W)0 : (W)(heat.t * heat.t * loss);
             }
+        } else {  // for every block of a cluster alike
+            if (helper && lane == 0 && team.part == 0) row_loss[row] = 0;
+            if (worker && g)
+                for (int v = v0 + lane; v < v1; v += 32) {
+                    Vec<T> z;
+#pragma unroll
+                    for (int u = 0; u < VEC; u++) z.e[u] = narrow<T>((W)0);
+                    sl.set(v, z);
+                }
         }
+        if (!few && wn != 0.0) team.sync_block();  // the slots have been read
+        if (worker) {
+            __syncwarp();
+            if (g) sl.store(v0, v1, lane, g);
+            if (wn != 0.0) ask(Slice<T>(row_mem, xs + next * ld, ncol, team.part, team.parts));
+            if (ONE) commit_copies();  // the row's; the slots' are the group before
+        }
+        if (helper && wn != 0.0) {
+            if (!few) ahead.load(te, next);
+            ahead.template work_out<ONE ? 1 : 0>(te, xs + next * ld, ncol, heat.inv, hash);
+        }
+        if (next >= nrow) break;
+        row = next;
+        w = wn;
+        set ^= 1;
     }
     if constexpr (CL) team.sync_all();  // a block stays while others may read its partials
 }
@@ -622,40 +767,62 @@ struct OnDevice {
     }
 };
 
+Heat heat_of(double t) {
+    Heat h;
+    h.t = t;
+    h.inv = 1.0 / t;
+    h.c = 16.0 * 1.4426950408889634 * h.inv;
+    h.cf = (float)(1.4426950408889634 * h.inv);
+    const auto high_word = [](double x) {
+        unsigned long long b;
+        memcpy(&b, &x, 8);
+        return (unsigned)(b >> 32);
+    };
+    h.high = (int)high_word(16000.0 / h.c);
+    h.low = high_word(-16300.0 / h.c);
+    return h;
+}
+
 // How a call's rows are dealt to threads.
 struct Deal {
-    int nt, parts;
+    int nt, help, parts, blocks;  // threads of a team (32: a warp) and its helper's, blocks of a team, of the grid
     size_t slice, team;  // bytes of shared memory: of a slice, of a team's part
 };
-constexpr size_t kSmemBlock = 227 * 1024;
+constexpr size_t kSmemBlock = 227 * 1024, kSmemSM = 228 * 1024;
 
 // Warps take short rows, blocks of 128 and 512 threads longer ones.  A row
 // that no block can hold is shared by a cluster of blocks, and one of few rows
 // too, so that the card is not left idle.
 template <typename T>
-Deal deal(const hx_readout* r, size_t extra, int sms) {
+Deal deal(const hx_readout* r, size_t extra, size_t warp_extra, int help, int sms) {
     Deal d{};
+    d.help = help;
     d.parts = 1;
-    if (r->ncol <= 512 && extra <= 6144) {
+    if (r->ncol <= 512 && extra <= warp_extra) {
         d.nt = 32;
     } else {
         while (d.parts < 8 && kRedBytes + Slice<T>::bytes(r->ncol, d.parts) + extra > kSmemBlock) d.parts *= 2;
         while (d.parts < 8 && (long long)r->nrow * d.parts * 2 <= sms && r->ncol / d.parts >= 4096) d.parts *= 2;
-        d.nt = d.parts == 1 && r->ncol <= 2048 ? 128 : 512;
+        d.nt = d.parts == 1 && r->ncol <= 2048 ? 128 : kBlock;
     }
     d.slice = Slice<T>::bytes(r->ncol, d.parts);
     d.team = kRedBytes + d.slice + (extra + 15) / 16 * 16;
+    // as many blocks as are resident at once: each takes rows in turn
+    const int rows = d.nt == 32 ? kWarpRows : 1;
+    const int per_sm = (int)std::min<size_t>(d.nt == kBlock ? 2 : 6, kSmemSM / (d.team * rows + 1024));
+    const long long all = ((long long)r->nrow + rows - 1) / rows * d.parts, most = (long long)sms * std::max(per_sm, 1) / d.parts * d.parts;
+    d.blocks = (int)std::min(all, most);
     return d;
 }
 
 template <typename... P, typename... A>
-cudaError_t launch(void (*kernel)(P...), const Deal& d, int nrow, cudaStream_t st, A... args) {
+cudaError_t launch(void (*kernel)(P...), const Deal& d, cudaStream_t st, A... args) {
     cudaLaunchConfig_t c{};
     c.dynamicSmemBytes = d.nt == 32 ? d.team * kWarpRows : d.team;
     if (c.dynamicSmemBytes > 48 * 1024)
         if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)c.dynamicSmemBytes)) return e;
-    c.gridDim = dim3(d.nt == 32 ? (unsigned)((nrow + kWarpRows - 1) / kWarpRows) : (unsigned)nrow * d.parts);
-    c.blockDim = dim3(d.nt == 32 ? 32 * kWarpRows : d.nt);
+    c.gridDim = dim3((unsigned)d.blocks);
+    c.blockDim = dim3(d.nt == 32 ? 32 * kWarpRows : d.nt + d.help);
     c.stream = st;
     cudaLaunchAttribute a;
     a.id = cudaLaunchAttributeClusterDimension;
@@ -735,13 +902,13 @@ int hx_distill_loss_grad_dev(hx_ctx* ctx, const hx_readout* rows, const hx_teach
         using T = std::remove_pointer_t<decltype(t)>;
         using W = typename Ty<T>::W;
         if (rows->nrow > 0) {
-            const Deal d = deal<T>(rows, distill_extra(teacher->k), sm_count(ctx->device));
+            const Deal d = deal<T>(rows, distill_extra(teacher->k), distill_extra(kFewSlots), 32, sm_count(ctx->device));
             auto go = [&](auto* kernel) {
-                return launch(kernel, d, rows->nrow, ctx->st, (const T*)rows->x, rows->nrow, rows->ncol, rows->ld, *teacher, temperature,
+                return launch(kernel, d, ctx->st, (const T*)rows->x, rows->nrow, rows->ncol, rows->ld, *teacher, heat_of(temperature),
                               scale, row_weight_dev, (T*)grad_dev, ld_grad, (W*)row_loss_dev, (int)d.team, (int)d.slice);
             };
-            HXC(d.nt == 32 ? go(distill_kernel<T, 32, false>) : d.parts > 1 ? go(distill_kernel<T, 512, true>)
-                : d.nt == 128 ? go(distill_kernel<T, 128, false>) : go(distill_kernel<T, 512, false>));
+            HXC(d.nt == 32 ? go(distill_kernel<T, 32, false>) : d.parts > 1 ? go(distill_kernel<T, kBlock, true>)
+                : d.nt == 128 ? go(distill_kernel<T, 128, false>) : go(distill_kernel<T, kBlock, false>));
         }
         loss_kernel<W><<<1, kThreads, 0, ctx->st>>>((const W*)row_loss_dev, row_weight_dev, rows->nrow, scale, (W*)loss_dev);
         HXC(cudaGetLastError());

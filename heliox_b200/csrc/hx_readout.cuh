@@ -75,51 +75,113 @@ __device__ __forceinline__ double load_any(const void* p, int dtype, size_t i) {
     }
 }
 
-// exp(d / T) for d <= 0: fp64 by the library's exp, fp32 by the hardware's 2^x
-// (about 2 steps of 2^-23; results below 2^-126 are 0).
+// exp((x - m) / T), m a readout near the largest.
+//
+// fp64: the table-driven method of P. T. P. Tang (ACM TOMS 15, 1989): with
+// d = x - m and s = 16 d log2(e) / T = 16 k + j + f, |f| <= 1/2, the result is
+// 2^k 2^(j/16) 2^(f/16), the last factor by a polynomial through the Chebyshev
+// nodes of degree 6 (relative error 1.5e-17).  The table holds 2^(j/16) less
+// j 2^-4 in the exponent's place, so that one addition of the whole number
+// 16 k + j puts the power of two in.  11 fp64 operations and one table entry:
+// 16 doubles are one entry per pair of shared-memory banks, so lanes never
+// wait for one another; 64 entries would save two operations and cost four
+// more conflicts.  Below 2^-1022 it is 0; above 2^1000 (and for NaN) it is
+// about 2^1000, which the caller sees in the sum.
+// fp32: the hardware's 2^x (about 3 half steps); results below 2^-126 are 0.
+constexpr int kPowBytes = 16 * 8;
+__constant__ unsigned long long kPow16[16] = {
+    0x3ff0000000000000, 0x3fefb5586cf9890f, 0x3fef72b83c7d517b, 0x3fef387a6e756238, 0x3fef06fe0a31b715, 0x3feedea64c123422,
+    0x3feebfdad5362a27, 0x3feeab07dd485429, 0x3feea09e667f3bcd, 0x3feea11473eb0187, 0x3feeace5422aa0db, 0x3feec49182a3f090,
+    0x3feee89f995ad3ad, 0x3fef199bdd85529c, 0x3fef5818dcfba487, 0x3fefa4afa2a490da};
+struct Heat {  // a temperature, worked out on the host
+    double t, inv, c;  // c = 16 log2(e) / T
+    int high;          // high word of the largest d that is taken as it is
+    unsigned low;      // and of the d below which the result is 0
+    float cf;          // log2(e) / T
+};
 struct Scaler64 {
-    double inv;
-    __device__ explicit Scaler64(double temperature) : inv(1.0 / temperature) {}
-    __device__ __forceinline__ double operator()(double d) const { return exp(d * inv); }
+    double c, m, inv;
+    int high;
+    unsigned low;
+    const int2* pow16;  // kPow16 in shared memory
+    __device__ __forceinline__ Scaler64(const Heat& h, double m_, const char* table)
+        : c(h.c), m(m_), inv(h.inv), high(h.high), low(h.low), pow16((const int2*)table) {}
+    __device__ __forceinline__ double operator()(double x) const {
+        const double d0 = x - m;
+        const double d = __hiloint2double(min(__double2hiint(d0), high), __double2loint(d0));
+        const double y = __fma_rn(d, c, 6755399441055744.0);  // 1.5 2^52: the sum's low bits are s to the nearest whole number
+        const int k = __double2loint(y);
+        const double f = __fma_rn(d, c, 6755399441055744.0 - y);
+        double q = 0x1.430a1d08ec681p-37;
+        q = __fma_rn(q, f, 0x1.5d897e525c216p-30);
+        q = __fma_rn(q, f, 0x1.3b2ab6fb41213p-23);
+        q = __fma_rn(q, f, 0x1.c6b08d6f2a289p-17);
+        q = __fma_rn(q, f, 0x1.ebfbdff82c590p-11);
+        q = __fma_rn(q, f, 0x1.62e42fefa39f3p-5);
+        q = q * f;
+        const int2 t = pow16[k & 15];
+        const double p = __hiloint2double(t.y + (k << 16), t.x);
+        const double e = __fma_rn(p, q, p);
+        return (unsigned)__double2hiint(d) > low ? 0.0 : e;
+    }
+    __device__ __forceinline__ double z(double x) const { return (x - m) * inv; }  // of which it is the exponential
+    static constexpr double most = 0x1p500;  // a sum up to here has left no readout out
 };
 struct Scaler32 {
-    float inv;
-    __device__ explicit Scaler32(double temperature) : inv((float)(1.4426950408889634 / temperature)) {}
-    __device__ __forceinline__ float operator()(float d) const {
+    float c, m;
+    double inv;
+    __device__ __forceinline__ Scaler32(const Heat& h, float m_, const char*) : c(h.cf), m(m_), inv(h.inv) {}
+    __device__ __forceinline__ float operator()(float x) const {
         float r;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * inv));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"((x - m) * c));
         return r;
     }
+    __device__ __forceinline__ double z(double x) const { return (x - (double)m) * inv; }
+    static constexpr double most = 0x1p40;
 };
-__device__ __forceinline__ Scaler64 scaler(double, double temperature) { return Scaler64(temperature); }
-__device__ __forceinline__ Scaler32 scaler(float, double temperature) { return Scaler32(temperature); }
+__device__ __forceinline__ Scaler64 scaler(double m, const Heat& h, const char* table) { return Scaler64(h, m, table); }
+__device__ __forceinline__ Scaler32 scaler(float m, const Heat& h, const char* table) { return Scaler32(h, m, table); }
 
-__device__ __forceinline__ double max_num(double a, double b) { return fmax(a, b); }  // the number, where one is NaN
-__device__ __forceinline__ float max_num(float a, float b) { return fmaxf(a, b); }
+// The larger of a and b; a where b is NaN.
+__device__ __forceinline__ double larger(double a, double b) { return b > a ? b : a; }
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
 
-constexpr int kRedBytes = 2 * 16 * 32 + 2 * 32;  // two buffers of 16 warps' partials and of the block's
+// A team's scratch: two buffers of 16 warps' partials and of the block's, the
+// table of powers, numbers that one warp leaves for the others.
+constexpr int kPartials = 2 * 16 * 32 + 2 * 32;
+constexpr int kRedBytes = kPartials + kPowBytes + 16 * 8;
 
 // The threads that own a row.  NT = 32: a warp, kWarpRows rows per block;
-// otherwise a block of NT threads, CL: a cluster of such blocks.
+// otherwise the first NT threads of a block, CL: of each block of a cluster.
+// HELP: the block has one more warp, the helper, which meets the others at
+// every barrier of sync_block() and reduce().
 constexpr int kWarpRows = 4;
-template <int NT_, bool CL_>
+__device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+__device__ __forceinline__ void bar_arrive(int id, int n) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+template <int NT_, bool CL_, bool HELP_>
 struct Team {
-    static constexpr int NT = NT_, NW = NT_ / 32;
-    static constexpr bool CL = CL_;
-    int t;            // thread within this block's part of the team
+    static constexpr int NT = NT_, NW = NT_ / 32, THREADS = NT_ + (HELP_ ? 32 : 0);
+    static constexpr bool CL = CL_, HELP = HELP_;
+    int t;            // thread within this block's part of the team; the helper's are NT .. NT+31
     int part, parts;  // block within the cluster
     int parity = 0, parity_all = 0;
     char* red;  // kRedBytes of shared memory
 
+    // The table of powers is ready after the next barrier.
     __device__ explicit Team(char* scratch) : red(scratch) {
         t = NT == 32 ? threadIdx.x & 31 : threadIdx.x;
+        if (t < 16) ((unsigned long long*)(red + kPartials))[t] = kPow16[t];
         part = CL ? (int)cg::this_cluster().block_rank() : 0;
         parts = CL ? (int)cg::this_cluster().num_blocks() : 1;
     }
-    static __device__ __forceinline__ size_t row_of_block(int parts) {
-        return NT == 32 ? (size_t)blockIdx.x * kWarpRows + (threadIdx.x >> 5) : CL ? (size_t)blockIdx.x / parts : (size_t)blockIdx.x;
+    // rows are dealt to the teams of the grid in turn
+    __device__ __forceinline__ long long first_row() const {
+        return NT == 32 ? (long long)blockIdx.x * kWarpRows + (threadIdx.x >> 5) : CL ? blockIdx.x / parts : blockIdx.x;
     }
-    __device__ __forceinline__ void sync() const {
+    __device__ __forceinline__ long long row_step() const {
+        return NT == 32 ? (long long)gridDim.x * kWarpRows : CL ? gridDim.x / parts : gridDim.x;
+    }
+    __device__ __forceinline__ void sync_block() const {
         if constexpr (NT == 32)
             __syncwarp();
         else
@@ -129,8 +191,10 @@ struct Team {
         if constexpr (CL)
             cg::this_cluster().sync();
         else
-            sync();
+            sync_block();
     }
+    __device__ __forceinline__ const char* table() const { return red + kPartials; }
+    __device__ __forceinline__ double* notes() const { return (double*)(red + kPartials + kPowBytes); }
     template <typename V>
     __device__ __forceinline__ V* of(V* p, int rank) const {  // p in another member's shared memory
         if constexpr (CL) return cg::this_cluster().map_shared_rank(p, rank);
@@ -138,20 +202,29 @@ struct Team {
     }
     // Reductions: butterflies within warps, then over the warps' and the
     // blocks' partials in a fixed order, so that every thread holds the same
-    // bits and no timing shows.  One barrier each (two buffers in turn); all
-    // threads of the block, with ALL of the cluster, take part.
-    template <bool ALL, typename V, typename F>
+    // bits and no timing shows.  reduce(): over the block, one barrier;
+    // across(): over the cluster's blocks, one cluster barrier.  Two buffers in
+    // turn: a buffer is written again only after a barrier that follows its
+    // last reading.  The helper listens: it passes no value.
+    template <typename V, typename F>
     __device__ __forceinline__ V reduce(V v, F op) {
         static_assert(sizeof(V) <= 32, "partials are 32 bytes");
-        v = warp(v, op);
+        if (!HELP || t < NT) v = warp(v, op);
         if constexpr (NW > 1) {
             char* buf = red + parity * 16 * 32;
-            if ((t & 31) == 0) *(V*)(buf + (t >> 5) * 32) = v;
+            if ((t & 31) == 0 && (!HELP || t < NT)) *(V*)(buf + (t >> 5) * 32) = v;
             __syncthreads();
             v = *(const V*)(buf + ((t & 31) % NW) * 32);
+#pragma unroll
             for (int o = NW / 2; o > 0; o >>= 1) v = op(v, shfl(v, o));
+            parity ^= 1;
         }
-        if constexpr (CL && ALL) {
+        return v;
+    }
+    template <typename V, typename F>
+    __device__ __forceinline__ V across(V v, F op) {
+        static_assert(sizeof(V) <= 32, "partials are 32 bytes");
+        if constexpr (CL) {
             V* mine = (V*)(red + 2 * 16 * 32 + parity_all * 32);
             parity_all ^= 1;
             if (t == 0) *mine = v;
@@ -159,7 +232,6 @@ struct Team {
             v = *of(mine, 0);
             for (int r = 1; r < parts; r++) v = op(v, *of(mine, r));
         }
-        parity ^= 1;
         return v;
     }
     template <typename V>
@@ -178,15 +250,36 @@ struct Team {
         for (int o = 16; o > 0; o >>= 1) v = op(v, shfl(v, o));
         return v;
     }
-    __device__ __forceinline__ bool any(bool p) const {  // of this block's part; a barrier
-        if constexpr (NT == 32) {
-            __syncwarp();
-            return __any_sync(~0u, p);
-        } else {
-            return __syncthreads_or(p);
-        }
-    }
 };
+
+// Asynchronous copies into shared memory; wait_copies() waits for the thread's own.
+__device__ __forceinline__ void copy8(void* d, const void* g) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((unsigned)__cvta_generic_to_shared(d)), "l"(g) : "memory");
+}
+__device__ __forceinline__ void copy4(void* d, const void* g) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((unsigned)__cvta_generic_to_shared(d)), "l"(g) : "memory");
+}
+template <int GROUPS = 0>  // all but the latest GROUPS groups
+__device__ __forceinline__ void wait_copies() {
+    if constexpr (GROUPS == 0)
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    else
+        asm volatile("cp.async.wait_group %0;" ::"n"(GROUPS) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+// Bulk copies out of shared memory, by one thread for a warp: the warp's writes
+// are fenced first; bulk_read() waits until the memory has been read and may be
+// written again.  They pass the load-store unit by, which global stores of a
+// whole row would fill for thousands of cycles: shared-memory traffic and
+// shuffles of every warp on the SM would wait behind them.
+__device__ __forceinline__ void fence_bulk() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void bulk_store(void* g, const void* s, unsigned bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(g), "r"((unsigned)__cvta_generic_to_shared(s)), "r"(bytes)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 
 // This block's slice of a row in shared memory, in 16-byte vectors aligned as
 // in global memory: element i of the slice is e[phase + i].  What the first
@@ -198,49 +291,70 @@ struct Slice {
     const T* src;
     int first;  // position of element 0 in the row
     int n, phase, nv;
+    int lo, wholes;  // the vectors that the slice fills
+    int room;        // vectors that any row's slice may have
 
     __device__ Slice(T* smem, const T* row, int ncol, int part, int parts) : e(smem) {
         const int per = (ncol + parts - 1) / parts;
         first = min(part * per, ncol);
         n = min(per, ncol - first);
+        room = per / VEC + 2;
         src = row + first;
         phase = n > 0 ? (int)(((size_t)src & 15) / sizeof(T)) : 0;
         nv = (phase + n + VEC - 1) / VEC;
+        lo = phase > 0;
+        wholes = max((phase + n) / VEC - lo, 0);
     }
     static size_t bytes(int ncol, int parts) {  // of shared memory (host)
         const int per = (ncol + parts - 1) / parts;
         return (size_t)(per / VEC + 2) * 16;
     }
-    __device__ __forceinline__ bool whole(int v) const {
-        return v * VEC >= phase && (v + 1) * VEC <= phase + n;
+    // Starts the copy of vectors v0 .. v1-1 into shared memory, by a warp: 16
+    // bytes at a time, elementwise at the slice's edges, so that nothing
+    // outside the row is read.
+    __device__ __forceinline__ void load(int v0, int v1, int lane) const {
+        const int a = max(v0, lo), b = min(v1, lo + wholes);
+        const T* from = src + ((a + lane) * VEC - phase);
+        unsigned to = (unsigned)__cvta_generic_to_shared(e + (a + lane) * VEC);
+#pragma unroll 4
+        for (int v = a + lane; v < b; v += 32, from += 32 * VEC, to += 32 * 16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+        edges(v0, v1, lane, [&](int u) { e[u] = u >= phase && u < phase + n ? src[u - phase] : narrow<T>((typename Ty<T>::W)-INFINITY); });
     }
-    // Starts the copy into shared memory: 16 bytes at a time, elementwise at
-    // the edges, so that nothing outside the row is read.
-    template <int NT>
-    __device__ void load(int t) const {
-        for (int v = t; v < nv; v += NT) {
-            if (whole(v)) {
-                const unsigned d = (unsigned)__cvta_generic_to_shared(e + v * VEC);
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src + (v * VEC - phase)) : "memory");
-            } else {
-                for (int u = v * VEC; u < (v + 1) * VEC; u++)
-                    e[u] = u >= phase && u < phase + n ? src[u - phase] : narrow<T>((typename Ty<T>::W)-INFINITY);
-            }
+    // f(u) for the elements (from the first vector's start) of partial vectors among v0 .. v1-1
+    template <typename F>
+    __device__ __forceinline__ void edges(int v0, int v1, int lane, F f) const {
+        if (lane < 2) {
+            const int v = lane == 0 ? 0 : nv - 1;
+            if (v >= v0 && v < v1 && (unsigned)(v - lo) >= (unsigned)wholes && (lane == 0 || nv > 1))
+                for (int u = v * VEC; u < (v + 1) * VEC; u++) f(u);
         }
     }
-    static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+    // The vectors of a warp, a run of them: the same places in shared memory
+    // for every row of a call, however the rows are aligned.
+    template <int NW>
+    __device__ __forceinline__ int run(int warp) const {
+        return min(warp * ((room + NW - 1) / NW), nv);
+    }
     __device__ __forceinline__ Vec<T> get(int v) const { return *(const Vec<T>*)(e + v * VEC); }
     __device__ __forceinline__ void set(int v, const Vec<T>& x) const { *(Vec<T>*)(e + v * VEC) = x; }
-    // Writes f(v)'s elements to a row of global memory, vectors where it is aligned like the source.
-    template <int NT, typename F>
-    __device__ void store(int t, T* row, F f) const {
-        T* dst = row + first;
-        const bool aligned = (((size_t)dst ^ (size_t)src) & 15) == 0;
-        for (int v = t; v < nv; v += NT) {
-            const Vec<T> x = f(v);
-            if (aligned && whole(v)) {
-                *(Vec<T>*)(dst + (v * VEC - phase)) = x;
-            } else {
+    // Vectors v0 .. v1-1 to this slice's place in a row of global memory, by a
+    // warp: in one bulk copy where the place is aligned like the source.
+    __device__ __forceinline__ void store(int v0, int v1, int lane, T* row) const {
+        T* const dst = row + first;
+        if ((((size_t)dst ^ (size_t)src) & 15) == 0) {
+            fence_bulk();
+            __syncwarp();
+            const int a = max(v0, lo), b = min(v1, lo + wholes);
+            if (lane == 0 && a < b) bulk_store(dst + (a * VEC - phase), e + a * VEC, (unsigned)(b - a) * 16);
+            edges(v0, v1, lane, [&](int u) {
+                if (u >= phase && u < phase + n) dst[u - phase] = e[u];
+            });
+            if (lane == 0) bulk_read();
+            __syncwarp();
+        } else {
+            for (int v = v0 + lane; v < v1; v += 32) {
+                const Vec<T> x = get(v);
 #pragma unroll
                 for (int u = 0; u < VEC; u++) {
                     const int i = v * VEC + u - phase;

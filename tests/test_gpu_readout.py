@@ -31,7 +31,8 @@ pytestmark = pytest.mark.gpu
 
 DT = {"f64": torch.float64, "f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 HALF = {"f64": 2.0**-53, "f32": 2.0**-24, "f16": 2.0**-11, "bf16": 2.0**-8}
-TINY = {"f64": 0.0, "f32": 2.0**-126, "f16": 2.0**-25, "bf16": 2.0**-126}  # fp32 exponentials below 2^-126 are 0; fp16: half a subnormal step
+# exponentials below 2^-1018 (fp64) and 2^-126 (fp32) of one whose sum is at least 1 are 0, here times a factor below 2^10; fp16: half a subnormal step
+TINY = {"f64": 2.0**-1000, "f32": 2.0**-116, "f16": 2.0**-25, "bf16": 2.0**-116}
 STAT = {"f64": torch.float64, "f32": torch.float32, "f16": torch.float32, "bf16": torch.float32}
 
 
@@ -486,6 +487,23 @@ def test_distill_slots_without_mass(sim):
     # values far below the rest: q of 0 leaves a term out, whatever the readout
     x = np.array([[0.0, -np.inf, 1.0, 2.0]])
     check_distill(sim, x, np.array([[1, 3]]), np.array([[-5000.0, 0.25]]), None, 1.0, "f64", "f64")
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_distill_slots_far_from_the_largest(sim, dtype):
+    # the readouts in the slots far below, or far above, nearly all of the row, by more than the types' exponents hold
+    rng = np.random.default_rng(7)
+    for n in (33, 700, 9000):
+        x = rng.integers(-40, 40, (6, n)) * (0.25 if dtype in ("f16", "bf16") else 1.0)
+        x[4] -= 500.0
+        x[5] = np.where(np.arange(n) % 5 == 1, -np.inf, x[5])
+        order = np.argsort(x, axis=1, kind="stable")[:, :6]
+        order[3] = np.argsort(-x[3], kind="stable")[:6]
+        order[5, :3] = [1, 6, 11]  # closed readouts in the first slots
+        val = rng.standard_normal(order.shape)
+        val[5, :3] = -5e5  # of no probability
+        for T in (1.0, 0.04, 1e-4):
+            check_distill(sim, x, order, val * T, None, T, dtype, "f64", scale=1.0 / T)
 
 
 def test_distill_empty_shapes(sim):
