@@ -22,6 +22,9 @@ using namespace hxr;
 
 constexpr int kThreads = 256;
 constexpr int kBlock = 256;  // threads of a block that has a row, or a slice of one, to itself (short rows: 128)
+template <typename T>
+constexpr int kBlocks = sizeof(T) == 8 ? 2 : 3;  // such blocks on an SM, where their shared memory lets them
+
 
 __device__ __forceinline__ void put(double* p, double v) { *p = v; }
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
@@ -240,9 +243,9 @@ size_t distill_extra(int k) { return (size_t)slot_list(k) * 20 * (k <= kFewSlots
 // (lane l has slots l, l + 32, ...).
 struct Slots {
     double* q;  // value, then probability
-    double* x;  // exponential of the row's readout there
+    double* x;  // the row's readout there, then its exponential
     int* at;    // position, -1: not used
-    double* notes;  // [0] log-sum-exp of the record, [1] sum of q, [2] sum of q log q, [3] 1: a slot is used, [4] a readout there
+    double* notes;  // [0] log-sum-exp of the record, [1] sum of q, [2] sum of q log q, [3] 1: a slot is used, [4] a readout there, [5], [6] of lifted(), [7] the largest value
     int lane;
     __device__ Slots(char* lists, double* all_notes, int k, int set, int thread) : lane(thread & 31) {
         q = (double*)(lists + (k <= kFewSlots ? set * slot_list(k) * 20 : 0));
@@ -274,9 +277,9 @@ struct Slots {
                 copy4(notes, (const float*)te.lse + row);
         }
     }
-    // Positions, probabilities and sums from the copied record; GROUPS of later copies may be on their way.
+    // The slots in use, from the copied record; GROUPS of later copies may be on their way.
     template <int GROUPS, typename T>
-    __device__ __forceinline__ void work_out(const hx_teacher& te, const T* row, int ncol, double inv, unsigned* hash) const {
+    __device__ __forceinline__ void sift(const hx_teacher& te, const T* row, int ncol, unsigned* hash) const {
         const int k = te.k, bits = hash_bits(k), most = 1 << bits;
         wait_copies<GROUPS>();
         if (k > 32)
@@ -329,21 +332,28 @@ struct Slots {
         }
         __syncwarp();
         const unsigned lanes = __ballot_sync(~0u, used);
-        T ref = narrow<T>((typename Ty<T>::W)0);
+        double ref = 0;
         if (lanes) {
             int j = __ffs(lanes) - 1;
             while (at[j] < 0) j += 32;  // that lane's first slot in use
-            ref = row[at[j]];
+            ref = (double)wide(row[at[j]]);
         }
-        double shift;
-        if (te.lse) {
-            shift = te.dtype == HX_DT_F64 ? notes[0] : (double)*(const float*)notes;
-            tm = 0;
-        } else {
+        if (!te.lse) {
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) tm = larger(tm, __shfl_xor_sync(~0u, tm, o));
-            shift = 0;
         }
+        if (lane == 0) {
+            notes[3] = lanes ? 1.0 : 0.0;
+            notes[4] = ref;
+            notes[7] = tm;
+        }
+    }
+    // Their probabilities and sums.
+    __device__ __forceinline__ void weigh(const hx_teacher& te, double inv) const {
+        const int k = te.k;
+        __syncwarp();
+        const double tm = te.lse ? 0.0 : notes[7];
+        const double shift = !te.lse ? 0.0 : te.dtype == HX_DT_F64 ? notes[0] : (double)*(const float*)notes;
         double s = 0, qv = 0;
         for (int j = lane; j < k; j += 32) {
             if (at[j] < 0) continue;
@@ -361,12 +371,28 @@ struct Slots {
             qv = qv * f - log(s);
             s = s == s ? 1.0 : s;
         }
-        __syncwarp();
         if (lane == 0) {
             notes[1] = s;
             notes[2] = qv;
-            notes[3] = lanes ? 1.0 : 0.0;
-            notes[4] = (double)wide(ref);
+        }
+    }
+    // The exponentials of the readouts that have been lifted out of this
+    // block's slice, and the sums of those and of q z.
+    template <typename T, typename E>
+    __device__ __forceinline__ void lifted(const Slice<T>& sl, int k, const E& ex) const {
+        double in = 0, qz = 0;
+        for (int j = lane; j < k; j += 32) {
+            if (at[j] < 0 || (unsigned)(at[j] - sl.first) >= (unsigned)sl.n) continue;
+            const double z = ex.z(x[j]), e = exp(z);
+            x[j] = e;
+            in += e;
+            qz += q[j] == 0.0 ? 0.0 : q[j] * z;
+        }
+        in = sum(in);
+        qz = sum(qz);
+        if (lane == 0) {
+            notes[5] = in;
+            notes[6] = qz;
         }
     }
     // f(j, cell) for the slots whose readouts are in vectors v0 .. v1-1 of the slice.
@@ -381,7 +407,7 @@ struct Slots {
 };
 
 template <typename T, int NT, bool CL>
-__global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT + 32, NT == kBlock ? 2 : 6)
+__global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT + 32, NT == kBlock ? kBlocks<T> : 6)
     distill_kernel(const T* xs, int nrow, int ncol, long long ld, hx_teacher te, Heat heat, double scale,
                    const double* __restrict__ weight, T* gs, long long ldg, typename Ty<T>::W* __restrict__ row_loss,
                    int team_bytes, int slice_bytes) {
@@ -415,7 +441,10 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT + 32, NT == kBl
         if (ONE) commit_copies();
         if (worker) ask(Slice<T>(row_mem, x, ncol, team.part, team.parts));
         if (ONE) commit_copies();
-        if (helper) slots.template work_out<ONE ? 1 : 0>(te, x, ncol, heat.inv, hash);
+        if (helper) {
+            slots.template sift<ONE ? 1 : 0>(te, x, ncol, hash);
+            slots.weigh(te, heat.inv);
+        }
     }
     for (;;) {
         const Slice<T> sl(row_mem, xs + row * ld, ncol, team.part, team.parts);
@@ -428,7 +457,11 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT + 32, NT == kBl
         if (worker) wait_copies();
         team.sync_block();  // the slots are ready, and those of the row before are free
         live = live && slots.notes[3] != 0.0;
-        // the next row's record, before the row's own traffic
+        // the next row into L2, its record into shared memory, before this row's own traffic
+        if (worker && wn != 0.0) {
+            const Slice<T> nx(row_mem, xs + next * ld, ncol, team.part, team.parts);
+            if (lane == 0) nx.prefetch(nx.template run<NW>(warp), nx.template run<NW>(warp + 1));
+        }
         if (helper && few && wn != 0.0) ahead.load(te, next);
         if (ONE) commit_copies();
         if (live) {
@@ -465,16 +498,14 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT + 32, NT == kBl
                     m = odd || empty ? (W)0 : top.mx;
                 }
                 const auto ex = scaler(m, heat, team.table());
-                s = Sums{0, 0, 0};
+                double out = 0;
                 if (worker) {
                     slots.each(sl, k, v0, v1, [&](int j, T* cell) {
-                        const double z = ex.z((double)wide(*cell)), e = exp(z), q = slots.q[j];
+                        slots.x[j] = (double)wide(*cell);
                         *cell = narrow<T>((W)-INFINITY);
-                        slots.x[j] = e;
-                        s.in += e;
-                        s.qz += q == 0.0 ? 0.0 : q * z;
                     });
                     __syncwarp();
+                    if (!ONE) bar_arrive(2, NT + 32);
                     W part[2] = {0, 0};
 #pragma unroll UNROLL
                     for (int v = v0 + lane; v < v1; v += 32) {
@@ -487,10 +518,17 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT + 32, NT == kBl
                         }
                         if constexpr (sizeof(T) == sizeof(W)) sl.set(v, x);
                     }
-                    s.out = (double)part[0] + (double)part[1];
+                    out = (double)part[0] + (double)part[1];
                 }
-                const auto op = [](Sums a, Sums b) { return Sums{a.out + b.out, a.in + b.in, a.qz + b.qz}; };
-                s = team.across(team.reduce(s, op), op);
+                if (helper) {
+                    if (!ONE) bar_sync(2, NT + 32);
+                    slots.lifted(sl, k, ex);
+                    if (!ONE && few && wn != 0.0 && !sure) ahead.template sift<0>(te, xs + next * ld, ncol, hash);
+                }
+                out = team.reduce(out, [](double a, double b) { return a + b; });
+                if (ONE) __syncwarp();
+                s = team.across(Sums{out, slots.notes[5], slots.notes[6]},
+                                [](Sums a, Sums b) { return Sums{a.out + b.out, a.in + b.in, a.qz + b.qz}; });
                 if (sure || (s.in + s.out <= decltype(ex)::most && s.in + s.out > 0.0)) break;
             }
             const double sum_q = slots.notes[1], sum_qlq = slots.notes[2];
@@ -543,7 +581,8 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT + 32, NT == kBl
         }
         if (helper && wn != 0.0) {
             if (!few) ahead.load(te, next);
-            ahead.template work_out<ONE ? 1 : 0>(te, xs + next * ld, ncol, heat.inv, hash);
+            if (ONE || !few || !live) ahead.template sift<ONE ? 1 : 0>(te, xs + next * ld, ncol, hash);
+            ahead.weigh(te, heat.inv);
         }
         if (next >= nrow) break;
         row = next;
@@ -553,17 +592,25 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT + 32, NT == kBl
     if constexpr (CL) team.sync_all();  // a block stays while others may read its partials
 }
 
+// scale sum_r w_r L_r in one block, each thread over rows of its own, then a tree: one order.
+constexpr int kLossThreads = 1024;
 template <typename W>
-__global__ void __launch_bounds__(kThreads) loss_kernel(const W* __restrict__ row_loss, const double* __restrict__ weight, int nrow,
-                                                        double scale, W* __restrict__ loss) {
-    __shared__ double red[kThreads];
+__global__ void __launch_bounds__(kLossThreads) loss_kernel(const W* __restrict__ row_loss, const double* __restrict__ weight, int nrow,
+                                                            double scale, W* __restrict__ loss) {
+    __shared__ double red[32];
     double s = 0;
-    for (int r = threadIdx.x; r < nrow; r += kThreads) {
-        const double w = weight ? weight[r] : 1.0;
-        if (w != 0.0) s += w * (double)row_loss[r];
+#pragma unroll 8
+    for (int r = threadIdx.x; r < nrow; r += kLossThreads) {
+        const double w = weight ? weight[r] : 1.0, l = (double)row_loss[r];
+        s += w != 0.0 ? w * l : 0.0;
     }
-    s = block_sum(s, red);
-    if (threadIdx.x == 0) *loss = (W)(scale * s);
+    s = Slots::sum(s);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        s = Slots::sum(red[threadIdx.x]);
+        if (threadIdx.x == 0) *loss = (W)(scale * s);
+    }
 }
 
 // ---------------------------------------------------------------- sampling
@@ -809,7 +856,7 @@ Deal deal(const hx_readout* r, size_t extra, size_t warp_extra, int help, int sm
     d.team = kRedBytes + d.slice + (extra + 15) / 16 * 16;
     // as many blocks as are resident at once: each takes rows in turn
     const int rows = d.nt == 32 ? kWarpRows : 1;
-    const int per_sm = (int)std::min<size_t>(d.nt == kBlock ? 2 : 6, kSmemSM / (d.team * rows + 1024));
+    const int per_sm = (int)std::min<size_t>(d.nt == kBlock ? kBlocks<T> : 6, kSmemSM / (d.team * rows + 1024));
     const long long all = ((long long)r->nrow + rows - 1) / rows * d.parts, most = (long long)sms * std::max(per_sm, 1) / d.parts * d.parts;
     d.blocks = (int)std::min(all, most);
     return d;
@@ -910,7 +957,7 @@ int hx_distill_loss_grad_dev(hx_ctx* ctx, const hx_readout* rows, const hx_teach
             HXC(d.nt == 32 ? go(distill_kernel<T, 32, false>) : d.parts > 1 ? go(distill_kernel<T, kBlock, true>)
                 : d.nt == 128 ? go(distill_kernel<T, 128, false>) : go(distill_kernel<T, kBlock, false>));
         }
-        loss_kernel<W><<<1, kThreads, 0, ctx->st>>>((const W*)row_loss_dev, row_weight_dev, rows->nrow, scale, (W*)loss_dev);
+        loss_kernel<W><<<1, kLossThreads, 0, ctx->st>>>((const W*)row_loss_dev, row_weight_dev, rows->nrow, scale, (W*)loss_dev);
         HXC(cudaGetLastError());
         return 0;
     });

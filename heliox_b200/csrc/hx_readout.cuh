@@ -321,6 +321,11 @@ struct Slice {
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
         edges(v0, v1, lane, [&](int u) { e[u] = u >= phase && u < phase + n ? src[u - phase] : narrow<T>((typename Ty<T>::W)-INFINITY); });
     }
+    // Vectors v0 .. v1-1 into L2.
+    __device__ __forceinline__ void prefetch(int v0, int v1) const {
+        const int a = max(v0, lo), b = min(v1, lo + wholes);
+        if (a < b) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src + (a * VEC - phase)), "r"((unsigned)(b - a) * 16) : "memory");
+    }
     // f(u) for the elements (from the first vector's start) of partial vectors among v0 .. v1-1
     template <typename F>
     __device__ __forceinline__ void edges(int v0, int v1, int lane, F f) const {
