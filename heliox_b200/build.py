@@ -12,13 +12,14 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libhx_b200.so")
 SOURCES = ["hx_kernels.cu", "hx_split.cu", "hx_runtime.cu", "hx_runtime_net.cu", "hx_runtime_lib.cu", "hx_netstim.cpp", "hx_plan.cpp", "hx_noalloc.cu",
-           "hx_readout.cu"]
+           "hx_readout.cu", "hx_select.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -42,7 +43,6 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return LIB
     objdir = os.path.join(HERE, "_build")
     os.makedirs(objdir, exist_ok=True)
-    objs = []
     common = [
         "-O3",
         "-std=c++17",
@@ -53,7 +53,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
         "-I" + os.path.join(ROOT, "include"),
         "-I" + CSRC,
     ] + ARCH
-    for src in SOURCES:
+
+    def compile_one(src: str) -> str:
         obj = os.path.join(objdir, src + ".o")
         cmd = [nvcc(), "-c", os.path.join(CSRC, src), "-o", obj] + common
         if verbose:
@@ -63,7 +64,10 @@ def build(force: bool = False, verbose: bool = False) -> str:
             raise RuntimeError(f"nvcc failed for {src}:\n{r.stdout}\n{r.stderr}")
         if verbose:
             sys.stderr.write(r.stderr)
-        objs.append(obj)
+        return obj
+
+    with ThreadPoolExecutor(max_workers=min(len(SOURCES), os.cpu_count() or 1)) as pool:
+        objs = list(pool.map(compile_one, SOURCES))
     tmp = LIB + ".tmp"
     cmd = [nvcc(), "-shared", "-o", tmp] + objs + ARCH + ["-cudart", "static", "-Xcompiler", "-fPIC"]
     r = subprocess.run(cmd, capture_output=True, text=True)

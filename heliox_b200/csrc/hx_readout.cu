@@ -1,16 +1,8 @@
-// hx_readout.cu -- operators over readout rows: a teacher's top logits, the
-// distillation loss of a student's rows with its gradient, sampled choices.
-//
-// One thread block per row; the row is read from global memory once per pass.
+// hx_readout.cu -- operators over readout rows: the distillation loss of a
+// student's rows with its gradient, and the C entries of all three.
 #include <cuda_runtime.h>
 
-#include <algorithm>
-#include <climits>
-#include <cmath>
-#include <cstdio>
-#include <cstring>
 #include <string>
-#include <type_traits>
 
 #include "heliox_b200.h"
 #include "hx_ctx.hpp"
@@ -19,194 +11,6 @@
 namespace {
 
 using namespace hxr;
-
-constexpr int kThreads = 256;
-constexpr int kBlock = 256;  // threads of a block that has a row, or a slice of one, to itself (short rows: 128)
-template <typename T>
-constexpr int kBlocks = sizeof(T) == 8 ? 2 : 3;  // such blocks on an SM, where their shared memory lets them
-
-
-__device__ __forceinline__ void put(double* p, double v) { *p = v; }
-__device__ __forceinline__ void put(float* p, float v) { *p = v; }
-__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-
-template <typename V, typename F>
-__device__ V block_reduce(V v, V* red, F op) {  // the same order whatever the timing
-    __syncthreads();
-    red[threadIdx.x] = v;
-    __syncthreads();
-    for (int s = kThreads / 2; s > 0; s >>= 1) {
-        if ((int)threadIdx.x < s) red[threadIdx.x] = op(red[threadIdx.x], red[threadIdx.x + s]);
-        __syncthreads();
-    }
-    return red[0];
-}
-template <typename V>
-__device__ V block_sum(V v, V* red) {
-    return block_reduce(v, red, [](V a, V b) { return a + b; });
-}
-template <typename V>
-__device__ V block_max(V v, V* red) {
-    return block_reduce(v, red, [](V a, V b) { return a > b ? a : b; });
-}
-
-// The border of the row's descending order at which a running measure (1 or
-// the mass of each element) first exceeds `target`: the border's key, and the
-// measure of everything above that key.  The caller makes sure that the whole
-// row's measure exceeds the target.
-template <typename T, typename M>
-__device__ typename Ty<T>::K select_border(const T* __restrict__ x, int n, unsigned long long target, M measure,
-                                           unsigned long long* above_out) {
-    using K = typename Ty<T>::K;
-    using W = typename Ty<T>::W;
-    __shared__ unsigned long long hist[256];
-    __shared__ int s_digit;
-    __shared__ unsigned long long s_above;
-    K prefix = 0, mask = 0;
-    unsigned long long above = 0;
-    for (int shift = (int)sizeof(K) * 8 - 8; shift >= 0; shift -= 8) {
-        __syncthreads();
-        hist[threadIdx.x] = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < n; i += kThreads) {
-            const W v = wide(x[i]);
-            if (v == -INFINITY) continue;
-            const K k = key_of(v);
-            if ((k & mask) != prefix) continue;
-            const unsigned long long m = measure(v);
-            if (m) atomicAdd(&hist[(int)((k >> shift) & 255)], m);
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            unsigned long long a = above;
-            int d = 255;
-            while (d > 0 && a + hist[d] <= target) a += hist[d--];
-            s_digit = d;
-            s_above = a;
-        }
-        __syncthreads();
-        above = s_above;
-        prefix |= (K)s_digit << shift;
-        mask |= (K)255 << shift;
-    }
-    *above_out = above;
-    return prefix;
-}
-
-// Calls take(i) for the first `want` elements of the row with this key, by position.
-template <typename T, typename F>
-__device__ void first_of_key(const T* __restrict__ x, int n, typename Ty<T>::K key, unsigned long long want, F take) {
-    __shared__ int wsum[kThreads / 32];
-    unsigned long long seen = 0;
-    for (int i0 = 0; i0 < n && seen < want; i0 += kThreads) {
-        const int i = i0 + threadIdx.x;
-        const bool hit = i < n && wide(x[i]) != -INFINITY && key_of(wide(x[i])) == key;
-        const unsigned b = __ballot_sync(~0u, hit);
-        if ((threadIdx.x & 31) == 0) wsum[threadIdx.x >> 5] = __popc(b);
-        __syncthreads();
-        unsigned long long at = seen + __popc(b & ((1u << (threadIdx.x & 31)) - 1));
-        int all = 0;
-        for (int w = 0; w < kThreads / 32; w++) {
-            if (w < (int)(threadIdx.x >> 5)) at += wsum[w];
-            all += wsum[w];
-        }
-        if (hit && at < want) take(i, at);
-        seen += all;
-        __syncthreads();
-    }
-}
-
-// ---------------------------------------------------------------- top logits
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) top_kernel(const T* __restrict__ xs, int ncol, long long ld, int k, double temperature,
-                                                       int* __restrict__ idx, T* __restrict__ val,
-                                                       typename Ty<T>::W* __restrict__ lse) {
-    using W = typename Ty<T>::W;
-    using K = typename Ty<T>::K;
-    __shared__ double red[kThreads];
-    __shared__ K skey[HX_READOUT_MAX_K];
-    __shared__ int sidx[HX_READOUT_MAX_K];
-    __shared__ int nabove;
-    const T* x = xs + (size_t)blockIdx.x * ld;
-    idx += (size_t)blockIdx.x * k;
-    val += (size_t)blockIdx.x * k;
-    W mx = -INFINITY;
-    int open = 0, bad = 0;
-    for (int i = threadIdx.x; i < ncol; i += kThreads) {
-        const W v = wide(x[i]);
-        if (v > mx) mx = v;
-        open += v > -INFINITY;
-        bad |= v != v;
-    }
-    mx = (W)block_max((double)mx, red);
-    open = block_sum(open, (int*)red);
-    bad = block_max(bad, (int*)red);
-    const W nan = (W)NAN;
-    if (lse) {
-        const W inv = (W)(1.0 / temperature);
-        W s = 0;
-        for (int i = threadIdx.x; i < ncol; i += kThreads) s += exp((wide(x[i]) - mx) * inv);
-        s = block_sum(s, (W*)red);
-        if (threadIdx.x == 0)
-            lse[blockIdx.x] = bad ? nan : mx == -INFINITY || mx == INFINITY ? mx : (W)((double)mx / temperature + log((double)s));
-    }
-    const int kk = bad ? 0 : min(k, open);
-    for (int j = kk + threadIdx.x; j < k; j += kThreads) {
-        idx[j] = -1;
-        put(&val[j], bad ? nan : (W)-INFINITY);
-    }
-    if (kk == 0) return;
-    unsigned long long above;
-    const K border = select_border(x, ncol, (unsigned long long)(kk - 1), [](W) { return 1ull; }, &above);
-    __syncthreads();
-    if (threadIdx.x == 0) nabove = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < ncol; i += kThreads) {
-        const W v = wide(x[i]);
-        if (v > -INFINITY && key_of(v) > border) {
-            const int at = atomicAdd(&nabove, 1);
-            skey[at] = key_of(v);
-            sidx[at] = i;
-        }
-    }
-    __syncthreads();
-    first_of_key(x, ncol, border, (unsigned long long)kk - above, [&](int i, unsigned long long at) {
-        skey[above + at] = border;
-        sidx[above + at] = i;
-    });
-    int p2 = 1;
-    while (p2 < kk) p2 <<= 1;
-    for (int j = kk + threadIdx.x; j < p2; j += kThreads) {
-        skey[j] = 0;
-        sidx[j] = INT_MAX;
-    }
-    for (int w = 2; w <= p2; w <<= 1) {
-        for (int d = w >> 1; d > 0; d >>= 1) {
-            __syncthreads();
-            for (int j = threadIdx.x; j < p2; j += kThreads) {
-                const int o = j ^ d;
-                if (o > j) {
-                    const K a = skey[j], b = skey[o];
-                    const int ia = sidx[j], ib = sidx[o];
-                    const bool first = a > b || (a == b && ia < ib);
-                    if (first != ((j & w) == 0)) {
-                        skey[j] = b;
-                        skey[o] = a;
-                        sidx[j] = ib;
-                        sidx[o] = ia;
-                    }
-                }
-            }
-        }
-    }
-    __syncthreads();
-    for (int j = threadIdx.x; j < kk; j += kThreads) {
-        idx[j] = sidx[j];
-        val[j] = x[sidx[j]];
-    }
-}
 
 // ---------------------------------------------------------------- distillation
 //
@@ -613,111 +417,6 @@ __global__ void __launch_bounds__(kLossThreads) loss_kernel(const W* __restrict_
     }
 }
 
-// ---------------------------------------------------------------- sampling
-
-struct Rule {
-    double temperature;
-    int top_k;
-    double top_p, min_p;
-};
-__device__ __forceinline__ Rule clean(const hx_sample_rule& r, int ncol) {
-    Rule o;
-    const bool greedy = r.temperature <= 0.0;
-    o.temperature = greedy ? 1.0 : r.temperature;
-    o.top_k = greedy ? 1 : r.top_k >= 1.0 ? (r.top_k < (double)ncol ? (int)r.top_k : ncol) : ncol;
-    o.top_p = r.top_p < 1.0 ? fmax(r.top_p, 0.0) : 1.0;
-    o.min_p = r.min_p > 0.0 ? fmin(r.min_p, 1.0) : 0.0;
-    return o;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const T* __restrict__ xs, int ncol, long long ld, hx_sample_rule rule,
-                                                          const hx_sample_rule* __restrict__ rules,
-                                                          const double* __restrict__ us, int bits, int* __restrict__ idx,
-                                                          typename Ty<T>::W* __restrict__ logp) {
-    using W = typename Ty<T>::W;
-    using K = typename Ty<T>::K;
-    __shared__ double red[kThreads];
-    __shared__ int s_at;
-    const T* x = xs + (size_t)blockIdx.x * ld;
-    const Rule r = clean(rules ? rules[blockIdx.x] : rule, ncol);
-    W mxw = -INFINITY;
-    int open = 0, bad = r.temperature != r.temperature;
-    for (int i = threadIdx.x; i < ncol; i += kThreads) {
-        const W v = wide(x[i]);
-        if (v > mxw) mxw = v;
-        open += v > -INFINITY;
-        bad |= v != v || v == INFINITY;
-    }
-    const double mx = block_max((double)mxw, red);
-    open = block_sum(open, (int*)red);
-    bad = block_max(bad, (int*)red);
-    if (bad || open == 0) {
-        if (threadIdx.x == 0) {
-            idx[blockIdx.x] = bad ? -2 : -1;
-            if (logp) logp[blockIdx.x] = bad ? (W)NAN : (W)-INFINITY;
-        }
-        return;
-    }
-    const double inv = 1.0 / r.temperature, unit = ldexp(1.0, bits);
-    auto weight = [&](W v) { return exp(((double)v - mx) * inv); };
-    auto mass = [&](W v) { return __double2ull_rn(weight(v) * unit); };
-    unsigned long long total, above;
-    const int top_k = min(r.top_k, open);
-    auto mass_above = [&](K key) {
-        unsigned long long s = 0;
-        for (int i = threadIdx.x; i < ncol; i += kThreads) {
-            const W v = wide(x[i]);
-            if (v > -INFINITY && key_of(v) > key) s += mass(v);
-        }
-        return block_sum(s, (unsigned long long*)red);
-    };
-    if (top_k < open) {
-        const K key = select_border(x, ncol, (unsigned long long)(top_k - 1), [](W) { return 1ull; }, &above);
-        total = mass_above(key) + ((unsigned long long)top_k - above) * mass(value_of(key));
-    } else {
-        total = mass_above(0);
-    }
-    double floor_ = r.min_p;  // kept: weight at least this
-    if (r.top_p < 1.0) {
-        const double want = ceil(r.top_p * (double)total);
-        unsigned long long target = want < 1.0 ? 1 : (unsigned long long)want;
-        if (target > total) target = total;
-        const K key = select_border(x, ncol, target - 1, mass, &above);
-        const W v = value_of(key);
-        const unsigned long long m = mass(v);
-        total = above + (target - above + m - 1) / m * m;
-        if (weight(v) >= floor_) floor_ = 0.0;
-    } else if (top_k < open) {
-        const K key = select_border(x, ncol, total - 1, mass, &above);
-        if (weight(value_of(key)) >= floor_) floor_ = 0.0;
-    }
-    if (floor_ > 0.0) {
-        unsigned long long s = 0;
-        for (int i = threadIdx.x; i < ncol; i += kThreads) {
-            const W v = wide(x[i]);
-            if (v > -INFINITY && weight(v) >= floor_) s += mass(v);
-        }
-        s = block_sum(s, (unsigned long long*)red);
-        total = s < total ? s : total;
-    }
-    double u = us[blockIdx.x];
-    u = u > 0.0 ? u : 0.0;
-    const double want = u < 1.0 ? floor(u * (double)total) : (double)total;
-    unsigned long long target = (unsigned long long)want;
-    if (target >= total) target = total - 1;
-    const K key = select_border(x, ncol, target, mass, &above);
-    const W v = value_of(key);
-    first_of_key(x, ncol, key, (target - above) / mass(v) + 1, [&](int i, unsigned long long at) {
-        if (at == (target - above) / mass(v)) s_at = i;
-    });
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        idx[blockIdx.x] = s_at;
-        if (logp) logp[blockIdx.x] = (W)(((double)v - mx) * inv - log((double)total / unit));
-    }
-}
-
 // ---------------------------------------------------------------- host side
 
 int type_size(int dtype) { return dtype == HX_DT_F64 ? 8 : dtype == HX_DT_F32 ? 4 : 2; }
@@ -814,89 +513,6 @@ struct OnDevice {
     }
 };
 
-Heat heat_of(double t) {
-    Heat h;
-    h.t = t;
-    h.inv = 1.0 / t;
-    h.c = 16.0 * 1.4426950408889634 * h.inv;
-    h.cf = (float)(1.4426950408889634 * h.inv);
-    const auto high_word = [](double x) {
-        unsigned long long b;
-        memcpy(&b, &x, 8);
-        return (unsigned)(b >> 32);
-    };
-    h.high = (int)high_word(16000.0 / h.c);
-    h.low = high_word(-16300.0 / h.c);
-    return h;
-}
-
-// How a call's rows are dealt to threads.
-struct Deal {
-    int nt, help, parts, blocks;  // threads of a team (32: a warp) and its helper's, blocks of a team, of the grid
-    size_t slice, team;  // bytes of shared memory: of a slice, of a team's part
-};
-constexpr size_t kSmemBlock = 227 * 1024, kSmemSM = 228 * 1024;
-
-// Warps take short rows, blocks of 128 and 512 threads longer ones.  A row
-// that no block can hold is shared by a cluster of blocks, and one of few rows
-// too, so that the card is not left idle.
-template <typename T>
-Deal deal(const hx_readout* r, size_t extra, size_t warp_extra, int help, int sms) {
-    Deal d{};
-    d.help = help;
-    d.parts = 1;
-    if (r->ncol <= 512 && extra <= warp_extra) {
-        d.nt = 32;
-    } else {
-        while (d.parts < 8 && kRedBytes + Slice<T>::bytes(r->ncol, d.parts) + extra > kSmemBlock) d.parts *= 2;
-        while (d.parts < 8 && (long long)r->nrow * d.parts * 2 <= sms && r->ncol / d.parts >= 4096) d.parts *= 2;
-        d.nt = d.parts == 1 && r->ncol <= 2048 ? 128 : kBlock;
-    }
-    d.slice = Slice<T>::bytes(r->ncol, d.parts);
-    d.team = kRedBytes + d.slice + (extra + 15) / 16 * 16;
-    // as many blocks as are resident at once: each takes rows in turn
-    const int rows = d.nt == 32 ? kWarpRows : 1;
-    const int per_sm = (int)std::min<size_t>(d.nt == kBlock ? kBlocks<T> : 6, kSmemSM / (d.team * rows + 1024));
-    const long long all = ((long long)r->nrow + rows - 1) / rows * d.parts, most = (long long)sms * std::max(per_sm, 1) / d.parts * d.parts;
-    d.blocks = (int)std::min(all, most);
-    return d;
-}
-
-template <typename... P, typename... A>
-cudaError_t launch(void (*kernel)(P...), const Deal& d, cudaStream_t st, A... args) {
-    cudaLaunchConfig_t c{};
-    c.dynamicSmemBytes = d.nt == 32 ? d.team * kWarpRows : d.team;
-    if (c.dynamicSmemBytes > 48 * 1024)
-        if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)c.dynamicSmemBytes)) return e;
-    c.gridDim = dim3((unsigned)d.blocks);
-    c.blockDim = dim3(d.nt == 32 ? 32 * kWarpRows : d.nt + d.help);
-    c.stream = st;
-    cudaLaunchAttribute a;
-    a.id = cudaLaunchAttributeClusterDimension;
-    a.val.clusterDim.x = d.parts;
-    a.val.clusterDim.y = a.val.clusterDim.z = 1;
-    if (d.parts > 1) {
-        c.attrs = &a;
-        c.numAttrs = 1;
-    }
-    return cudaLaunchKernelEx(&c, kernel, P(args)...);
-}
-
-int sm_count(int device) {
-    int n = 0;
-    return cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) == cudaSuccess ? n : 1;
-}
-
-template <typename F>
-int by_type(int dtype, F f) {
-    switch (dtype) {
-        case HX_DT_F64: return f((double*)nullptr);
-        case HX_DT_F32: return f((float*)nullptr);
-        case HX_DT_F16: return f((__half*)nullptr);
-        default: return f((__nv_bfloat16*)nullptr);
-    }
-}
-
 }  // namespace
 
 #define HXC(call)                                                                                       \
@@ -928,13 +544,8 @@ int hx_top_logits_dev(hx_ctx* ctx, const hx_readout* rows, int k, double tempera
     if (rows->nrow == 0) return 0;
     OnDevice on(ctx->device);
     HXC(on.e);
-    return by_type(rows->dtype, [&](auto* t) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        top_kernel<T><<<rows->nrow, kThreads, 0, ctx->st>>>((const T*)rows->x, rows->ncol, rows->ld, k, temperature, idx_dev,
-                                                            (T*)val_dev, (typename Ty<T>::W*)lse_dev);
-        HXC(cudaGetLastError());
-        return 0;
-    });
+    HXC(launch_top(*rows, k, heat_of(temperature), idx_dev, val_dev, lse_dev, sm_count(ctx->device), ctx->st));
+    return 0;
 }
 
 int hx_distill_loss_grad_dev(hx_ctx* ctx, const hx_readout* rows, const hx_teacher* teacher, double temperature,
@@ -949,7 +560,7 @@ int hx_distill_loss_grad_dev(hx_ctx* ctx, const hx_readout* rows, const hx_teach
         using T = std::remove_pointer_t<decltype(t)>;
         using W = typename Ty<T>::W;
         if (rows->nrow > 0) {
-            const Deal d = deal<T>(rows, distill_extra(teacher->k), distill_extra(kFewSlots), 32, sm_count(ctx->device));
+            const Deal d = deal<T>(*rows, distill_extra(teacher->k), distill_extra(kFewSlots), 32, sm_count(ctx->device));
             auto go = [&](auto* kernel) {
                 return launch(kernel, d, ctx->st, (const T*)rows->x, rows->nrow, rows->ncol, rows->ld, *teacher, heat_of(temperature),
                               scale, row_weight_dev, (T*)grad_dev, ld_grad, (W*)row_loss_dev, (int)d.team, (int)d.slice);
@@ -970,17 +581,12 @@ int hx_sample_dev(hx_ctx* ctx, const hx_readout* rows, const hx_sample_rule* rul
     if (rows->nrow == 0) return 0;
     int lg = 0;
     while ((1ll << lg) < rows->ncol) lg++;
-    const int bits = lg <= 10 ? 52 : 62 - lg;
+    const int bits = lg <= 10 ? 52 : 62 - lg;  // a row's masses add up to less than 2^62
     const hx_sample_rule none{1.0, 0.0, 1.0, 0.0};
     OnDevice on(ctx->device);
     HXC(on.e);
-    return by_type(rows->dtype, [&](auto* t) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        sample_kernel<T><<<rows->nrow, kThreads, 0, ctx->st>>>((const T*)rows->x, rows->ncol, rows->ld, rules_dev ? none : *rule,
-                                                               rules_dev, u_dev, bits, idx_dev, (typename Ty<T>::W*)logp_dev);
-        HXC(cudaGetLastError());
-        return 0;
-    });
+    HXC(launch_sample(*rows, rules_dev ? none : *rule, rules_dev, u_dev, bits, idx_dev, logp_dev, sm_count(ctx->device), ctx->st));
+    return 0;
 }
 
 }  // extern "C"

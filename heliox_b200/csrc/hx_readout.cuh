@@ -12,6 +12,13 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <cstdio>
+#include <cstring>
+#include <type_traits>
+
 #include "heliox_b200.h"
 
 namespace hxr {
@@ -369,5 +376,99 @@ struct Slice {
         }
     }
 };
+
+// ---------------------------------------------------------------- host side
+
+constexpr int kBlock = 256;  // threads of a block that has a row, or a slice of one, to itself (short rows: 128)
+template <typename T>
+constexpr int kBlocks = sizeof(T) == 8 ? 2 : 3;  // such blocks on an SM, where their shared memory lets them
+
+inline Heat heat_of(double t) {
+    Heat h;
+    h.t = t;
+    h.inv = 1.0 / t;
+    h.c = 16.0 * 1.4426950408889634 * h.inv;
+    h.cf = (float)(1.4426950408889634 * h.inv);
+    const auto high_word = [](double x) {
+        unsigned long long b;
+        memcpy(&b, &x, 8);
+        return (unsigned)(b >> 32);
+    };
+    h.high = (int)high_word(16000.0 / h.c);
+    h.low = high_word(-16300.0 / h.c);
+    return h;
+}
+
+// How a call's rows are dealt to threads.
+struct Deal {
+    int nt, help, parts, blocks;  // threads of a team (32: a warp) and its helper's, blocks of a team, of the grid
+    size_t slice, team;  // bytes of shared memory: of a slice, of a team's part
+};
+constexpr size_t kSmemBlock = 227 * 1024, kSmemSM = 228 * 1024;
+
+// Warps take short rows, blocks of 128 and 512 threads longer ones.  A row
+// that no block can hold is shared by a cluster of blocks, and one of few rows
+// too, so that the card is not left idle.
+template <typename T>
+Deal deal(const hx_readout& r, size_t extra, size_t warp_extra, int help, int sms) {
+    Deal d{};
+    d.help = help;
+    d.parts = 1;
+    if (r.ncol <= 512 && extra <= warp_extra) {
+        d.nt = 32;
+    } else {
+        while (d.parts < 8 && kRedBytes + Slice<T>::bytes(r.ncol, d.parts) + extra > kSmemBlock) d.parts *= 2;
+        while (d.parts < 8 && (long long)r.nrow * d.parts * 2 <= sms && r.ncol / d.parts >= 4096) d.parts *= 2;
+        d.nt = d.parts == 1 && r.ncol <= 2048 ? 128 : kBlock;
+    }
+    d.slice = Slice<T>::bytes(r.ncol, d.parts);
+    d.team = kRedBytes + d.slice + (extra + 15) / 16 * 16;
+    // as many blocks as are resident at once: each takes rows in turn
+    const int rows = d.nt == 32 ? kWarpRows : 1;
+    const int per_sm = (int)std::min<size_t>(d.nt == kBlock ? kBlocks<T> : 6, kSmemSM / (d.team * rows + 1024));
+    const long long all = ((long long)r.nrow + rows - 1) / rows * d.parts, most = (long long)sms * std::max(per_sm, 1) / d.parts * d.parts;
+    d.blocks = (int)std::min(all, most);
+    return d;
+}
+
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), const Deal& d, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t c{};
+    c.dynamicSmemBytes = d.nt == 32 ? d.team * kWarpRows : d.team;
+    if (c.dynamicSmemBytes > 48 * 1024)
+        if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)c.dynamicSmemBytes)) return e;
+    c.gridDim = dim3((unsigned)d.blocks);
+    c.blockDim = dim3(d.nt == 32 ? 32 * kWarpRows : d.nt + d.help);
+    c.stream = st;
+    cudaLaunchAttribute a;
+    a.id = cudaLaunchAttributeClusterDimension;
+    a.val.clusterDim.x = d.parts;
+    a.val.clusterDim.y = a.val.clusterDim.z = 1;
+    if (d.parts > 1) {
+        c.attrs = &a;
+        c.numAttrs = 1;
+    }
+    return cudaLaunchKernelEx(&c, kernel, P(args)...);
+}
+
+inline int sm_count(int device) {
+    int n = 0;
+    return cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) == cudaSuccess ? n : 1;
+}
+
+template <typename F>
+auto by_type(int dtype, F f) {
+    switch (dtype) {
+        case HX_DT_F64: return f((double*)nullptr);
+        case HX_DT_F32: return f((float*)nullptr);
+        case HX_DT_F16: return f((__half*)nullptr);
+        default: return f((__nv_bfloat16*)nullptr);
+    }
+}
+
+// hx_select.cu
+cudaError_t launch_top(const hx_readout& rows, int k, const Heat& heat, int* idx, void* val, void* lse, int sms, cudaStream_t st);
+cudaError_t launch_sample(const hx_readout& rows, const hx_sample_rule& rule, const hx_sample_rule* rules, const double* u, int bits,
+                          int* idx, void* logp, int sms, cudaStream_t st);
 
 }  // namespace hxr

@@ -623,9 +623,10 @@ int hx_distill_loss_grad_dev(hx_ctx* ctx, const hx_readout* rows, const hx_teach
  * statistics, may be NULL): the log of its probability within the run (-inf and
  * NaN beside -1 and -2).  Probabilities count in units of 2^-s of the largest
  * one, s = min(52, 62 - log2 ncol rounded up).  In rules_dev a temperature
- * below or at 0 takes the largest, a share top_p outside (0, 1) is 1 above and
- * leaves the largest alone below, min_p is held to [0, 1], NaN in the three
- * switches that cut off; u outside [0, 1) is held to it, NaN is 0. */
+ * below 1e-30 takes the largest and one above 1e30 is 1e30, a share top_p
+ * outside (0, 1) is 1 above and leaves the largest alone below, min_p is held
+ * to [0, 1], NaN in the three switches that cut off; u outside [0, 1) is held
+ * to it, NaN is 0. */
 int hx_sample_dev(hx_ctx* ctx, const hx_readout* rows, const hx_sample_rule* rule, const hx_sample_rule* rules_dev,
                   const double* u_dev, int32_t* idx_dev, void* logp_dev);
 

@@ -646,6 +646,24 @@ def test_sample_frequencies(sim):
 
 # ------------------------------------------------------------------ calls as programs make them
 
+@pytest.mark.parametrize("dtype", ["f64", "bf16"])
+@pytest.mark.parametrize("nrow", [8, 90])
+def test_long_rows_of_equal_readouts(sim, dtype, nrow):
+    # rows shared by several blocks (few rows) and rows of a block (many): more equal readouts than any list of candidates holds
+    rng = np.random.default_rng(17)
+    n = 20011
+    a = np.stack([np.full(n, -65.0), rng.integers(0, 3, n) * 1.0, np.where(rng.random(n) < 0.9, -np.inf, 0.0),
+                  np.where(np.arange(n) < 40, rng.permutation(n) * 1e-3, -65.0), np.where(np.arange(n) % 2, -65.0, -65.5),
+                  rng.standard_normal(n), np.full(n, -np.inf), np.where(np.arange(n) == n - 1, np.nan, 1.0)])
+    x = np.concatenate([a, np.tile(rng.standard_normal((1, n)), (nrow - 8, 1))]) if nrow > 8 else a
+    check_top(sim, x, 100, 1.0, dtype)
+    u = rng.random(nrow)
+    for rule in (dict(), dict(top_p=0.6180339), dict(top_k=64, top_p=0.6180339), dict(top_k=3000), dict(temperature=0.01, min_p=0.017), dict(temperature=0.0)):
+        check_sample(sim, x, u, dtype, **rule)
+    order, val, lse = teacher(rng, np.where(np.isfinite(x), x, 0.0), 30, 1.0, True)
+    check_distill(sim, x, order, val, lse, 1.0, dtype, "f64", scale=10.0)
+
+
 def test_same_bits_twice_and_whatever_the_batch(sim):
     rng = np.random.default_rng(2)
     for dtype, n in (("f64", 302), ("f64", 9001), ("bf16", 30011), ("f32", 120)):
