@@ -20,12 +20,20 @@ struct Bag {   // candidates
     int* count;
     int cap;
 };
-constexpr int kBins = 256;  // counting bins of the distance from the row's largest readout
-
-// Distances d = largest - x >= 0 fall into bins of an eighth of an octave,
-// from below 2^-16 to above 2^16.
-__device__ __forceinline__ int bin_of(float d) { return min(max((int)(__float_as_uint(d) >> 20) - 888, 0), kBins - 1); }
-__device__ __forceinline__ float bin_end(int b) { return b >= kBins - 1 ? INFINITY : __uint_as_float((unsigned)(889 + b) << 20); }
+// Distances d = largest - x >= 0 are counted in bins from below 2^-16 to above
+// 2^16: 32 of an octave for a block, 16 for a warp, which has fewer readouts.
+template <int NT>
+constexpr int kBins = NT == 32 ? 512 : 1024;
+template <int NT>
+constexpr int kMantissa = NT == 32 ? 4 : 5;  // bits of a distance's mantissa that number its bin
+template <int NT>
+__device__ __forceinline__ int bin_of(float d) {
+    return min(max((int)(__float_as_uint(d) >> (23 - kMantissa<NT>)) - (111 << kMantissa<NT>), 0), kBins<NT> - 1);
+}
+template <int NT>
+__device__ __forceinline__ float bin_end(int b) {
+    return b >= kBins<NT> - 1 ? INFINITY : __uint_as_float((unsigned)((111 << kMantissa<NT>) + 1 + b) << (23 - kMantissa<NT>));
+}
 template <typename W>
 __device__ __forceinline__ float distance(W top, W x) {  // also where both are +inf
     return x == top ? 0.0f : (float)(top - x);
@@ -43,32 +51,55 @@ __device__ __forceinline__ u64 scan(u64 v, int lane) {  // inclusive, over a war
     return v;
 }
 
-// The row's largest readout, NaN left out, and whether one is NaN (or, with
-// INF, +inf).
+// The larger of two; NaN where one is NaN (fp64: b where a is NaN).
+__device__ __forceinline__ double larger_nan(double a, double b) { return b > a ? b : a; }
+__device__ __forceinline__ float larger_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// The largest of a vector's elements, NaN where one is NaN (but not in fp64): 16-bit types two at a time.
+__device__ __forceinline__ double of_vector(const Vec<double>& x) { return larger_nan(x.e[0], x.e[1]); }
+__device__ __forceinline__ float of_vector(const Vec<float>& x) {
+    return larger_nan(larger_nan(x.e[0], x.e[1]), larger_nan(x.e[2], x.e[3]));
+}
+__device__ __forceinline__ float of_vector(const Vec<__half>& x) {
+    const __half2* p = (const __half2*)x.e;
+    const __half2 m = __hmax2_nan(__hmax2_nan(p[0], p[1]), __hmax2_nan(p[2], p[3]));
+    return larger_nan(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ float of_vector(const Vec<__nv_bfloat16>& x) {
+    const __nv_bfloat162* p = (const __nv_bfloat162*)x.e;
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(p[0], p[1]), __hmax2_nan(p[2], p[3]));
+    return larger_nan(__low2float(m), __high2float(m));
+}
+
+// The row's largest readout, and whether a readout is NaN (odd 1) or +inf (odd 2; also 1 alone where one is NaN).
 template <typename W>
 struct Top {
     W mx;
     int odd;
 };
-template <bool INF, typename T, typename G>
+template <typename T, typename G>
 __device__ __forceinline__ Top<typename Ty<T>::W> largest(G& team, const Slice<T>& sl, int v0, int v1, int lane) {
     using W = typename Ty<T>::W;
-    Top<W> t{(W)-INFINITY, 0};
-#pragma unroll 2
+    W mx = -INFINITY;
+    bool fine = true;
+#pragma unroll 4
     for (int v = v0 + lane; v < v1; v += 32) {
         const Vec<T> x = sl.get(v);
-#pragma unroll
-        for (int u = 0; u < Ty<T>::VEC; u++) {
-            const W y = wide(x.e[u]);
-            t.mx = larger(t.mx, y);
-            if (INF)
-                t.odd |= !(y < (W)INFINITY);
-            else
-                t.odd |= y != y;
+        if constexpr (sizeof(W) == 8) {
+            fine &= (x.e[0] == x.e[0]) & (x.e[1] == x.e[1]);
+            mx = larger(larger(mx, x.e[0]), x.e[1]);
+        } else {
+            mx = larger_nan(mx, of_vector(x));
         }
     }
+    Top<W> t{mx, (mx == mx && fine ? 0 : 1) | (mx == (W)INFINITY ? 2 : 0)};
+    if (mx != mx) t.mx = -INFINITY;
     const auto op = [](Top<W> a, Top<W> b) { return Top<W>{larger(a.mx, b.mx), a.odd | b.odd}; };
-    return team.across(team.reduce(t, op), op);
+    t = team.across(team.reduce(t, op), op);
+    return t;
 }
 
 // ---------------------------------------------------------------- the k largest
@@ -80,41 +111,44 @@ __device__ __forceinline__ Top<typename Ty<T>::W> largest(G& team, const Slice<T
 // into is gathered.
 
 // Each lane's vectors in groups; each group's maximum is counted in the
-// leading block's histogram.  f(value) sees every readout.
+// leading block's histogram.  f(vector) sees every vector.
 template <typename T, typename G, typename F>
 __device__ __forceinline__ void count_groups(G& team, const Slice<T>& sl, int v0, int v1, int lane, int ncol, int k,
                                              typename Ty<T>::W top, unsigned* hist, F f) {
     using W = typename Ty<T>::W;
     constexpr int VEC = Ty<T>::VEC;
     unsigned* const h = team.of(hist, 0);
-    const bool each = ncol < 2 * k * VEC;                        // too few vectors: every readout is a group
-    const int per = each ? 1 : max(1, ncol / (4 * k * VEC));  // vectors of a group
-    W g = -INFINITY;
-    int left = per;
-    for (int v = v0 + lane; v < v1; v += 32) {
-        const Vec<T> x = sl.get(v);
+    if (ncol < 2 * k * VEC) {  // too few vectors: every readout is a group
+        for (int v = v0 + lane; v < v1; v += 32) {
+            const Vec<T> x = sl.get(v);
+            f(x);
 #pragma unroll
-        for (int u = 0; u < VEC; u++) {
-            const W y = wide(x.e[u]);
-            f(y);
-            g = larger(g, y);
-            if (each) {
-                if (y > (W)-INFINITY) atomicAdd(h + bin_of(distance(top, y)), 1u);
+            for (int u = 0; u < VEC; u++) {
+                const W y = wide(x.e[u]);
+                if (y > (W)-INFINITY) atomicAdd(h + bin_of<G::NT>(distance(top, y)), 1u);
             }
         }
-        if (--left == 0 || v + 32 >= v1) {
-            if (!each && g > (W)-INFINITY) atomicAdd(h + bin_of(distance(top, g)), 1u);
-            g = -INFINITY;
-            left = per;
+        return;
+    }
+    const int per = max(1, ncol / (4 * k * VEC));  // vectors of a group
+    for (int v = v0 + lane; v < v1;) {
+        W g = -INFINITY;
+        const int end = min(v1, v + 32 * per);
+#pragma unroll 2
+        for (; v < end; v += 32) {
+            const Vec<T> x = sl.get(v);
+            f(x);
+            g = larger(g, of_vector(x));
         }
+        if (g > (W)-INFINITY) atomicAdd(h + bin_of<G::NT>(distance(top, g)), 1u);
     }
 }
 
 // The bin that the k-th group falls into (the last bin where there are fewer), by the leading block's threads.
 template <typename G>
 __device__ __forceinline__ void find_bin(G& team, const unsigned* hist, int k, int* bin) {
-    constexpr int PER = kBins / G::NT;
-    static_assert(PER * G::NT == kBins, "");
+    constexpr int PER = kBins<G::NT> / G::NT;
+    static_assert(PER * G::NT == kBins<G::NT>, "");
     const int t = team.t;
     unsigned c[PER], s = 0;
 #pragma unroll
@@ -133,16 +167,18 @@ __device__ __forceinline__ void find_bin(G& team, const unsigned* hist, int k, i
     }
 }
 
-// Puts every readout of this block's slice for which want(value) into the leading block's bag.
-template <typename T, typename G, typename K, typename F>
-__device__ __forceinline__ void gather(G& team, const Slice<T>& sl, int v0, int v1, int lane, const Bag<K>& bag, F want) {
+// Puts every readout of this block's slice for which want(value) into the
+// leading block's bag; vectors for which maybe(vector) is false have none.
+template <typename T, typename G, typename K, typename P, typename F>
+__device__ __forceinline__ void gather(G& team, const Slice<T>& sl, int v0, int v1, int lane, const Bag<K>& bag, P maybe, F want) {
     constexpr int VEC = Ty<T>::VEC;
     K* const key = team.of(bag.key, 0);
     int *const pos = team.of(bag.pos, 0), *const count = team.of(bag.count, 0);
     const int at = sl.first - sl.phase;
-#pragma unroll 2
+#pragma unroll 4
     for (int v = v0 + lane; v < v1; v += 32) {
         const Vec<T> x = sl.get(v);
+        if (!maybe(x)) continue;
 #pragma unroll
         for (int u = 0; u < VEC; u++) {
             const auto y = wide(x.e[u]);
@@ -156,6 +192,17 @@ __device__ __forceinline__ void gather(G& team, const Slice<T>& sl, int v0, int 
         }
     }
 }
+// Those in the bins up to b.  What reaches the least value of these bins, or
+// comes a rounding short of it, is taken: a few too many do no harm.
+template <typename T, typename G, typename K>
+__device__ __forceinline__ void gather_bins(G& team, const Slice<T>& sl, int v0, int v1, int lane, const Bag<K>& bag, int b, typename Ty<T>::W top) {
+    using W = typename Ty<T>::W;
+    W least = top - (W)bin_end<G::NT>(b) * (W)1.000001;
+    const W lowest = sizeof(W) == 8 ? (W)-1.7976931348623157e308 : (W)-3.4028234663852886e38f;
+    if (b >= kBins<G::NT> - 1 || !(least > lowest)) least = lowest;
+    if (top == (W)INFINITY && b < kBins<G::NT> - 1) least = top;
+    gather<T>(team, sl, v0, v1, lane, bag, [&](const Vec<T>& x) { return !(of_vector(x) < least); }, [&](W y) { return y >= least; });
+}
 
 // The n candidates in order: put(rank, key, position) for the first `want`, by
 // one block's threads.  Few are ranked by comparing each with all others, more
@@ -164,7 +211,7 @@ template <typename G, typename K, typename F>
 __device__ __forceinline__ void in_order(G& team, const Bag<K>& bag, int n, int want, F put) {
     constexpr int NT = G::NT;
     const int t = team.t;
-    if (n <= (NT == 32 ? 64 : 256)) {
+    if (n <= (NT == 32 ? 64 : 128)) {
         for (int j = t; j < n; j += NT) {
             const K k = bag.key[j];
             const int p = bag.pos[j];
@@ -294,10 +341,12 @@ __device__ void first_of_key(G& team, const T* __restrict__ x, int n, u64 key, u
 
 // ---------------------------------------------------------------- top logits
 
-size_t top_extra(int cap, size_t key) { return kSlowBytes + 16 + (size_t)cap * (key + 4); }
-int top_cap(int k) {
+template <int NT>
+constexpr int kCountBytes = kBins<NT> * 4 > kSlowBytes ? kBins<NT> * 4 : kSlowBytes;
+size_t top_extra(int nt, int cap, size_t key) { return (nt == 32 ? kCountBytes<32> : kCountBytes<kBlock>)+16 + (size_t)cap * (key + 4); }
+int top_cap(int k) {  // room for the candidates: a power of two
     int c = 128;
-    while (c < 2 * k) c *= 2;
+    while (c < 3 * k && c < 2 * HX_READOUT_MAX_K) c *= 2;
     return c;
 }
 
@@ -315,9 +364,9 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ?
     T* const row_mem = (T*)(mine + kRedBytes);
     char* const extra = mine + kRedBytes + slice_bytes;
     unsigned* const hist = (unsigned*)extra;  // and the digits of find_border()
-    int* const count = (int*)(extra + kSlowBytes);
+    int* const count = (int*)(extra + kCountBytes<NT>);
     int* const bin = count + 1;
-    const Bag<K> bag{(K*)(extra + kSlowBytes + 16), (int*)((K*)(extra + kSlowBytes + 16) + cap), count, cap};
+    const Bag<K> bag{(K*)(extra + kCountBytes<NT> + 16), (int*)((K*)(extra + kCountBytes<NT> + 16) + cap), count, cap};
     const bool lead = team.part == 0;
     const long long step = team.row_step();
     long long row = team.first_row();
@@ -326,42 +375,49 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ?
         const Slice<T> s(row_mem, xs + r * ld, ncol, team.part, team.parts);
         s.load(s.template run<NW>(warp), s.template run<NW>(warp + 1), lane);
     };
+    const auto prefetch = [&](long long r) {
+        const Slice<T> s(row_mem, xs + r * ld, ncol, team.part, team.parts);
+        if (lane == 0) s.prefetch(s.template run<NW>(warp), s.template run<NW>(warp + 1));
+    };
     ask(row);
     for (;;) {
         const T* const x = xs + row * ld;
         const Slice<T> sl(row_mem, x, ncol, team.part, team.parts);
         const int v0 = sl.template run<NW>(warp), v1 = sl.template run<NW>(warp + 1);
         const long long next = row + step;
-        for (int b = t; b < kBins; b += NT) hist[b] = 0;
+        for (int b = t; b < kBins<NT>; b += NT) hist[b] = 0;
         if (t == 0) {
             *count = 0;
-            *bin = kBins - 1;
+            *bin = kBins<NT> - 1;
         }
         wait_copies();
+        if (next < nrow) prefetch(next);
         if (NT == 32) __syncwarp();
-        const Top<W> top = largest<false, T>(team, sl, v0, v1, lane);
+        const Top<W> top = largest<T>(team, sl, v0, v1, lane);
         if (NT == 32) __syncwarp();
         int* const out_idx = idx + row * k;
         T* const out_val = val + row * k;
         int n = 0;
-        if (!top.odd && top.mx > (W)-INFINITY) {
+        const bool odd = top.odd & 1;
+        if (!odd && top.mx > (W)-INFINITY) {
             double sum = 0;
             if (lse) {
                 const auto ex = scaler(top.mx, heat, team.table());
                 W part = 0;
-                count_groups<T>(team, sl, v0, v1, lane, ncol, k, top.mx, hist, [&](W y) { part += ex(y); });
+                count_groups<T>(team, sl, v0, v1, lane, ncol, k, top.mx, hist, [&](const Vec<T>& xv) {
+#pragma unroll
+                    for (int q = 0; q < Ty<T>::VEC; q++) part += ex(wide(xv.e[q]));
+                });
                 sum = team.reduce((double)part, [](double a, double b) { return a + b; });
             } else {
-                count_groups<T>(team, sl, v0, v1, lane, ncol, k, top.mx, hist, [](W) {});
+                count_groups<T>(team, sl, v0, v1, lane, ncol, k, top.mx, hist, [](const Vec<T>&) {});
             }
             sum = team.across(sum, [](double a, double b) { return a + b; });
             if (!CL) team.sync_block();
             if (lead) find_bin(team, hist, k, bin);
             team.sync_all();
             const int b = *team.of(bin, 0);
-            const float end = bin_end(b);
-            const bool all = b == kBins - 1;
-            gather<T>(team, sl, v0, v1, lane, bag, [&](W y) { return y > (W)-INFINITY && (all || distance(top.mx, y) < end); });
+            gather_bins<T>(team, sl, v0, v1, lane, bag, b, top.mx);
             team.sync_all();
             if (next < nrow) ask(next);
             if (lead) {
@@ -394,12 +450,12 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ?
             }
         } else {
             if (next < nrow) ask(next);
-            if (lse && lead && t == 0) lse[row] = top.odd ? (W)NAN : (W)-INFINITY;
+            if (lse && lead && t == 0) lse[row] = odd ? (W)NAN : (W)-INFINITY;
         }
         if (lead)
             for (int j = min(n, k) + t; j < k; j += NT) {
                 out_idx[j] = -1;
-                out_val[j] = narrow<T>(top.odd ? (W)NAN : (W)-INFINITY);
+                out_val[j] = narrow<T>(odd ? (W)NAN : (W)-INFINITY);
             }
         if (next >= nrow) break;
         row = next;
@@ -474,16 +530,27 @@ struct Scale {
     }
 };
 
+constexpr int kParts = 128;  // of a bin, where it has many readouts
 constexpr int kMassBins = 896;  // 16 * (52 + 2) and more
 template <int NT>
 constexpr int kCoarse = NT == 32 ? 2 : 0;  // a warp's bins are four times as wide
 template <int NT>
 constexpr int kRowBins = kMassBins >> kCoarse<NT>;
 
+template <int NT>
+constexpr int kMassBytes = kRowBins<NT> * 8 > kCountBytes<NT> ? kRowBins<NT> * 8 : kCountBytes<NT>;
 static_assert(128 * (8 + 4 + 4 + 4) >= kSlowBytes, "find_border() has the candidates' place");
 size_t sample_extra(int nt, int cap, size_t key) {
-    const size_t bins = (size_t)(nt == 32 ? kRowBins<32> : kMassBins) * 8;
-    return std::max<size_t>(bins, kSlowBytes) + 64 + (size_t)cap * (key + 4) + (size_t)cap * (8 + 4);
+    const size_t lists = (size_t)cap * (key + 4) + (size_t)cap * (8 + 4);
+    return nt == 32 ? kMassBytes<32> + 64 + lists : kMassBytes<kBlock> + 64 + lists + (size_t)cap * (key + 4) + kParts * 8;
+}
+
+// Adds a mass to a bin (two words) in shared memory: the carry goes with the high word.
+__device__ __forceinline__ void add_mass(unsigned at, u64 m) {
+    const unsigned lo = (unsigned)m;
+    unsigned was;
+    asm volatile("atom.shared.add.u32 %0, [%1], %2;" : "=r"(was) : "r"(at), "r"(lo) : "memory");
+    asm volatile("red.shared.add.u32 [%0], %1;" ::"r"(at + 4), "r"((unsigned)(m >> 32) + (was + lo < was ? 1u : 0u)) : "memory");
 }
 
 // The first of n masses in order (running sums cum) whose running mass exceeds target; by a warp.
@@ -515,14 +582,16 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ?
     unsigned* const hist = (unsigned*)extra;  // counting bins, or
     uint2* const bins = (uint2*)extra;        // masses of the bins (low and high words), then the masses before each, or
     u64* const digits = (u64*)extra;          // of find_border()
-    char* const rest = extra + (NB * 8 > kSlowBytes ? NB * 8 : kSlowBytes);
+    char* const rest = extra + kMassBytes<NT>;
     u64* const found = (u64*)rest;  // [0] mass before the bin, [1] its number, [2] total mass, [3] key of the choice
     int* const count = (int*)(found + 4);
     int* const bin = count + 1;
-    int* const choice = count + 2;
+    int *const choice = count + 2, *const count2 = count + 3;
     u64* const cum = (u64*)(rest + 64);  // running masses of the candidates in order
     const Bag<K> bag{(K*)(cum + cap), (int*)((K*)(cum + cap) + cap), count, cap};
     int* const pos = bag.pos + cap;  // positions in order; keys in order: in cum's place until the masses are
+    uint2* const parts = (uint2*)(pos + cap);  // NT > 32: masses of the parts of a bin, and the readouts of one part
+    const Bag<K> fine{(K*)(parts + kParts), (int*)((K*)(parts + kParts) + cap), count2, cap};
     const bool lead = team.part == 0;
     const long long step = team.row_step();
     long long row = team.first_row();
@@ -530,6 +599,10 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ?
     const auto ask = [&](long long r) {
         const Slice<T> s(row_mem, xs + r * ld, ncol, team.part, team.parts);
         s.load(s.template run<NW>(warp), s.template run<NW>(warp + 1), lane);
+    };
+    const auto prefetch = [&](long long r) {
+        const Slice<T> s(row_mem, xs + r * ld, ncol, team.part, team.parts);
+        if (lane == 0) s.prefetch(s.template run<NW>(warp), s.template run<NW>(warp + 1));
     };
     ask(row);
     for (;;) {
@@ -541,14 +614,15 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ?
         double u = us[row];
         const Rule r = clean(given, ncol);
         const bool few = r.top_k < ncol && r.top_k <= cap / 2, by_mass = r.top_k >= ncol;
-        for (int b = t; b < NB * 2 || b < kBins; b += NT) hist[b] = 0;
+        for (int b = t; b < NB * 2 || b < kBins<NT>; b += NT) hist[b] = 0;
         if (t == 0) {
             *count = 0;
-            *bin = kBins - 1;
+            *bin = kBins<NT> - 1;
         }
         wait_copies();
+        if (next < nrow) prefetch(next);
         if (NT == 32) __syncwarp();
-        const Top<W> top = largest<true, T>(team, sl, v0, v1, lane);
+        const Top<W> top = largest<T>(team, sl, v0, v1, lane);
         if (NT == 32) __syncwarp();
         const bool odd = top.odd || given.temperature != given.temperature;
         if (odd || top.mx == (W)-INFINITY) {
@@ -585,14 +659,12 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ?
                 return s;
             };
             if (few) {
-                count_groups<T>(team, sl, v0, v1, lane, ncol, r.top_k, top.mx, hist, [](W) {});
+                count_groups<T>(team, sl, v0, v1, lane, ncol, r.top_k, top.mx, hist, [](const Vec<T>&) {});
                 team.sync_all();
                 if (lead) find_bin(team, hist, r.top_k, bin);
                 team.sync_all();
                 const int b = *team.of(bin, 0);
-                const float end = bin_end(b);
-                const bool all = b == kBins - 1;
-                gather<T>(team, sl, v0, v1, lane, bag, [&](W y) { return y > (W)-INFINITY && (all || distance(top.mx, y) < end); });
+                gather_bins<T>(team, sl, v0, v1, lane, bag, b, top.mx);
                 team.sync_all();
                 if (next < nrow) ask(next);
                 if (lead) {
@@ -652,6 +724,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ?
                 }
             } else if (by_mass) {
                 u64 atleast = 0;
+                const unsigned bins_at = (unsigned)__cvta_generic_to_shared(bins);
 #pragma unroll 2
                 for (int v = v0 + lane; v < v1; v += 32) {
                     const Vec<T> xv = sl.get(v);
@@ -661,9 +734,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ?
                         if (s > sc.least) {
                             const double e = sc.weight(s);
                             const u64 m = sc.mass_of(e);
-                            uint2* const b = bins + (-__double2loint(Scale::rounded(s)) >> kCoarse<NT>);
-                            const unsigned lo = (unsigned)m, was = atomicAdd(&b->x, lo), hi = (unsigned)(m >> 32) + (was + lo < was);
-                            if (hi) atomicAdd(&b->y, hi);
+                            add_mass(bins_at + (-__double2loint(Scale::rounded(s)) >> kCoarse<NT>) * 8, m);
                             if (r.min_p > 0.0 && e >= r.min_p) atleast += m;
                         }
                     }
@@ -720,6 +791,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ?
                             }
                         }
                         if (t == 0) *count = 0;
+                        if (NW > 1 && t < kParts) parts[t] = make_uint2(0, 0);
                     }
                     team.sync_all();
                     const int b = *team.of(bin, 0);
@@ -727,13 +799,69 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ?
                         const double s = sc.arg((double)y);
                         return s > sc.least && -__double2loint(Scale::rounded(s)) >> kCoarse<NT> == b;
                     };
-                    gather<T>(team, sl, v0, v1, lane, bag, in);
+                    // every readout of the bin lies between these
+                    const double width = (double)(1 << kCoarse<NT>) / sc.c, far = (double)(b + 1) * width;
+                    const W hi = (W)(sc.m - ((double)b - 1.0) * width), lo = (W)(sc.m - far);
+                    gather<T>(team, sl, v0, v1, lane, bag,
+                              [&](const Vec<T>& xv) {
+                                  bool some = false;
+#pragma unroll
+                                  for (int q = 0; q < Ty<T>::VEC; q++) some |= (wide(xv.e[q]) <= hi) & (wide(xv.e[q]) >= lo);
+                                  return some;
+                              },
+                              in);
                     team.sync_all();
                     if (last && next < nrow) ask(next);
                     if (lead) {
-                        const int n = *count;
-                        const u64 above = found[0];
+                        int n = *count;
+                        u64 above = found[0];
+                        Bag<K> list = bag;
                         team.sync_block();
+                        if constexpr (NW > 1) {
+                            if (n > 64 && n <= cap) {  // by the fraction of the argument: one of kParts parts of the bin
+                                const auto part_of = [&](double v) {
+                                    const double s = sc.arg(v);
+                                    return min(max((int)((0.5 - (s - (Scale::rounded(s) - 6755399441055744.0))) * kParts), 0), kParts - 1);
+                                };
+                                const unsigned parts_at = (unsigned)__cvta_generic_to_shared(parts);
+                                for (int j = t; j < n; j += NT) {
+                                    const double v = (double)value_of(bag.key[j]);
+                                    add_mass(parts_at + part_of(v) * 8, sc.mass(v));
+                                }
+                                team.sync_block();
+                                if (t < 32) {
+                                    constexpr int P = kParts / 32;
+                                    u64 m[P], s = 0;
+#pragma unroll
+                                    for (int i = 0; i < P; i++) {
+                                        const uint2 w = parts[lane * P + i];
+                                        s += m[i] = (u64)w.y << 32 | w.x;
+                                    }
+                                    u64 a = above + scan(s, lane) - s;
+#pragma unroll
+                                    for (int i = 0; i < P; i++) {
+                                        if (a <= target && target < a + m[i]) {
+                                            found[0] = a;
+                                            *choice = lane * P + i;
+                                        }
+                                        a += m[i];
+                                    }
+                                    if (lane == 0) *count2 = 0;
+                                }
+                                team.sync_block();
+                                const int one = *choice;
+                                above = found[0];
+                                for (int j = t; j < n; j += NT)
+                                    if (part_of((double)value_of(bag.key[j])) == one) {
+                                        const int p = atomicAdd(count2, 1);
+                                        fine.key[p] = bag.key[j];
+                                        fine.pos[p] = bag.pos[j];
+                                    }
+                                team.sync_block();
+                                n = *count2;
+                                list = fine;
+                            }
+                        }
                         if (n > cap) {
                             const Border br = find_border(team, x, ncol, cum, target, above, in, [&](W y) { return sc.mass((double)y); });
                             const u64 m = sc.mass((double)value_of((K)br.key)), nth = (target - br.above) / m;
@@ -744,7 +872,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ?
                             at.through = br.above + (nth + 1) * m;
                             at.pos = *choice;
                         } else {
-                            in_order(team, bag, n, n, [&](int j, K key, int p) {
+                            in_order(team, list, n, n, [&](int j, K key, int p) {
                                 cum[j] = (u64)key;
                                 pos[j] = p;
                             });
@@ -841,7 +969,9 @@ cudaError_t launch_top(const hx_readout& rows, int k, const Heat& heat, int* idx
         using T = std::remove_pointer_t<decltype(tag)>;
         const int cap = top_cap(k);
         const size_t key = sizeof(typename Ty<T>::K);
-        const Deal d = deal<T>(rows, top_extra(cap, key), top_extra(256, key), 0, sms);
+        const bool warps = rows.ncol <= 512 && cap <= 512;
+        const size_t ex = top_extra(warps ? 32 : kBlock, cap, key);
+        const Deal d = deal<T>(rows, ex, warps ? ex : 0, 0, sms);
         const auto go = [&](auto* kernel) {
             return launch(kernel, d, st, (const T*)rows.x, rows.nrow, rows.ncol, rows.ld, k, heat, idx, (T*)val, (typename Ty<T>::W*)lse, cap,
                           (int)d.team, (int)d.slice);
@@ -859,7 +989,9 @@ cudaError_t launch_sample(const hx_readout& rows, const hx_sample_rule& rule, co
         // room for twice top_k where it is known and small; per-row rules: up to 256
         int cap = rows.ncol <= 512 ? 128 : 512;
         if (!rules)
-            while (cap < 1024 && rule.top_k >= 1.0 && 2.0 * rule.top_k > cap) cap *= 2;
+            while (cap < 1024 && rule.top_k >= 1.0 && 2.0 * rule.top_k > cap &&
+                   kRedBytes + Slice<T>::bytes(rows.ncol, 8) + sample_extra(kBlock, 2 * cap, key) <= kSmemBlock)
+                cap *= 2;
         const bool warps = rows.ncol <= 512 && cap <= 256;
         const size_t ex = sample_extra(warps ? 32 : kBlock, cap, key);
         const Deal d = deal<T>(rows, ex, warps ? ex : 0, 0, sms);
