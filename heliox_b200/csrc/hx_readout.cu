@@ -32,6 +32,10 @@ using namespace hxr;
 // a block of many warps by a helper, which has no run, so that its chain of
 // dependent exponentials and reductions is waited for by nobody.
 
+constexpr int kBlock = 256;  // threads of a block that has a row, or a slice of one, to itself (short rows: 128)
+template <typename T>
+constexpr int kBlocks = sizeof(T) == 8 ? 2 : 3;  // such blocks on an SM, where their shared memory lets them
+
 constexpr int kFewSlots = 128;  // up to here the next row's slots are worked out into lists of their own
 
 __host__ __device__ constexpr int slot_list(int k) { return (k + 3) / 4 * 4; }
@@ -560,7 +564,7 @@ int hx_distill_loss_grad_dev(hx_ctx* ctx, const hx_readout* rows, const hx_teach
         using T = std::remove_pointer_t<decltype(t)>;
         using W = typename Ty<T>::W;
         if (rows->nrow > 0) {
-            const Deal d = deal<T>(*rows, distill_extra(teacher->k), distill_extra(kFewSlots), 32, sm_count(ctx->device));
+            const Deal d = deal<T>(*rows, distill_extra(teacher->k), distill_extra(kFewSlots), kBlock, kBlocks<T>, 32, sm_count(ctx->device));
             auto go = [&](auto* kernel) {
                 return launch(kernel, d, ctx->st, (const T*)rows->x, rows->nrow, rows->ncol, rows->ld, *teacher, heat_of(temperature),
                               scale, row_weight_dev, (T*)grad_dev, ld_grad, (W*)row_loss_dev, (int)d.team, (int)d.slice);

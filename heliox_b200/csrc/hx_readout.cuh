@@ -379,10 +379,6 @@ struct Slice {
 
 // ---------------------------------------------------------------- host side
 
-constexpr int kBlock = 256;  // threads of a block that has a row, or a slice of one, to itself (short rows: 128)
-template <typename T>
-constexpr int kBlocks = sizeof(T) == 8 ? 2 : 3;  // such blocks on an SM, where their shared memory lets them
-
 inline Heat heat_of(double t) {
     Heat h;
     h.t = t;
@@ -410,7 +406,7 @@ constexpr size_t kSmemBlock = 227 * 1024, kSmemSM = 228 * 1024;
 // that no block can hold is shared by a cluster of blocks, and one of few rows
 // too, so that the card is not left idle.
 template <typename T>
-Deal deal(const hx_readout& r, size_t extra, size_t warp_extra, int help, int sms) {
+Deal deal(const hx_readout& r, size_t extra, size_t warp_extra, int block, int blocks, int help, int sms) {
     Deal d{};
     d.help = help;
     d.parts = 1;
@@ -419,13 +415,13 @@ Deal deal(const hx_readout& r, size_t extra, size_t warp_extra, int help, int sm
     } else {
         while (d.parts < 8 && kRedBytes + Slice<T>::bytes(r.ncol, d.parts) + extra > kSmemBlock) d.parts *= 2;
         while (d.parts < 8 && (long long)r.nrow * d.parts * 2 <= sms && r.ncol / d.parts >= 4096) d.parts *= 2;
-        d.nt = d.parts == 1 && r.ncol <= 2048 ? 128 : kBlock;
+        d.nt = d.parts == 1 && r.ncol <= 2048 ? 128 : block;
     }
     d.slice = Slice<T>::bytes(r.ncol, d.parts);
     d.team = kRedBytes + d.slice + (extra + 15) / 16 * 16;
     // as many blocks as are resident at once: each takes rows in turn
     const int rows = d.nt == 32 ? kWarpRows : 1;
-    const int per_sm = (int)std::min<size_t>(d.nt == kBlock ? kBlocks<T> : 6, kSmemSM / (d.team * rows + 1024));
+    const int per_sm = (int)std::min<size_t>(d.nt == block ? blocks : 6, kSmemSM / (d.team * rows + 1024));
     const long long all = ((long long)r.nrow + rows - 1) / rows * d.parts, most = (long long)sms * std::max(per_sm, 1) / d.parts * d.parts;
     d.blocks = (int)std::min(all, most);
     return d;

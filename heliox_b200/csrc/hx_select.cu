@@ -12,6 +12,11 @@ using namespace hxr;
 
 using u64 = unsigned long long;
 
+constexpr int kWide = 256;  // threads of a block that has a row, or a slice of one, to itself (short rows: 128)
+template <typename T>
+constexpr int kWides = sizeof(T) == 8 ? 2 : 3;  // such blocks on an SM, where their shared memory lets them
+
+
 // What a team needs besides the row, in its leading block's shared memory.
 template <typename K>
 struct Bag {   // candidates
@@ -169,24 +174,48 @@ __device__ __forceinline__ void find_bin(G& team, const unsigned* hist, int k, i
 
 // Puts every readout of this block's slice for which want(value) into the
 // leading block's bag; vectors for which maybe(vector) is false have none.
+// Hits are rare: lanes first mark the vectors that may have some, then count
+// theirs, and the warp takes its places in the bag with one atomic addition.
 template <typename T, typename G, typename K, typename P, typename F>
 __device__ __forceinline__ void gather(G& team, const Slice<T>& sl, int v0, int v1, int lane, const Bag<K>& bag, P maybe, F want) {
     constexpr int VEC = Ty<T>::VEC;
     K* const key = team.of(bag.key, 0);
     int *const pos = team.of(bag.pos, 0), *const count = team.of(bag.count, 0);
     const int at = sl.first - sl.phase;
+    for (int first = v0; first < v1; first += 32 * 32) {
+        const int mine = min(32, (v1 - first - lane + 31) >> 5);  // vectors of this lane
+        unsigned marks = 0;
 #pragma unroll 4
-    for (int v = v0 + lane; v < v1; v += 32) {
-        const Vec<T> x = sl.get(v);
-        if (!maybe(x)) continue;
+        for (int i = 0; i < mine; i++)
+            if (maybe(sl.get(first + lane + 32 * i))) marks |= 1u << i;
+        if (!__any_sync(~0u, marks)) continue;
+        int hits = 0;
+        for (unsigned m = marks; m; m &= m - 1) {
+            const Vec<T> x = sl.get(first + lane + 32 * (__ffs(m) - 1));
 #pragma unroll
-        for (int u = 0; u < VEC; u++) {
-            const auto y = wide(x.e[u]);
-            if (want(y)) {
-                const int p = atomicAdd(count, 1);
-                if (p < bag.cap) {
-                    key[p] = key_of(y);
-                    pos[p] = at + v * VEC + u;
+            for (int u = 0; u < VEC; u++) hits += want(wide(x.e[u]));
+        }
+        int upto = hits;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int h = __shfl_up_sync(~0u, upto, o);
+            if (lane >= o) upto += h;
+        }
+        int p = 0;
+        if (lane == 31) p = atomicAdd(count, upto);
+        p = __shfl_sync(~0u, p, 31) + upto - hits;
+        for (unsigned m = hits ? marks : 0u; m; m &= m - 1) {
+            const int v = first + lane + 32 * (__ffs(m) - 1);
+            const Vec<T> x = sl.get(v);
+#pragma unroll
+            for (int u = 0; u < VEC; u++) {
+                const auto y = wide(x.e[u]);
+                if (want(y)) {
+                    if (p < bag.cap) {
+                        key[p] = key_of(y);
+                        pos[p] = at + v * VEC + u;
+                    }
+                    p++;
                 }
             }
         }
@@ -205,12 +234,34 @@ __device__ __forceinline__ void gather_bins(G& team, const Slice<T>& sl, int v0,
 }
 
 // The n candidates in order: put(rank, key, position) for the first `want`, by
-// one block's threads.  Few are ranked by comparing each with all others, more
-// by a bitonic network in place.
+// one block's threads.  Few are ranked by comparing each with all others (with
+// ranks, kRanks zeroed numbers, by all threads of a block), more by a bitonic
+// network in place.
+constexpr int kRanks = 128;
 template <typename G, typename K, typename F>
-__device__ __forceinline__ void in_order(G& team, const Bag<K>& bag, int n, int want, F put) {
+__device__ __forceinline__ void in_order(G& team, const Bag<K>& bag, int n, int want, int* ranks, F put) {
     constexpr int NT = G::NT;
     const int t = team.t;
+    if constexpr (NT > 32) {
+        if (ranks && n > 32 && n <= kRanks) {  // each by several threads
+            int p2 = 64;
+            while (p2 < n) p2 <<= 1;
+            const int j = t & (p2 - 1), groups = NT / p2, each = (n + groups - 1) / groups;
+            const int l0 = (t / p2) * each, l1 = min(l0 + each, n);
+            K k = 0;
+            int p = 0, r = 0;
+            if (j < n) {
+                k = bag.key[j];
+                p = bag.pos[j];
+#pragma unroll 4
+                for (int l = l0; l < l1; l++) r += before(bag.key[l], bag.pos[l], k, p);
+                if (r) atomicAdd(ranks + j, r);
+            }
+            team.sync_block();
+            if (t < n && ranks[t] < want) put(ranks[t], k, p);
+            return;
+        }
+    }
     if (n <= (NT == 32 ? 64 : 128)) {
         for (int j = t; j < n; j += NT) {
             const K k = bag.key[j];
@@ -343,7 +394,7 @@ __device__ void first_of_key(G& team, const T* __restrict__ x, int n, u64 key, u
 
 template <int NT>
 constexpr int kCountBytes = kBins<NT> * 4 > kSlowBytes ? kBins<NT> * 4 : kSlowBytes;
-size_t top_extra(int nt, int cap, size_t key) { return (nt == 32 ? kCountBytes<32> : kCountBytes<kBlock>)+16 + (size_t)cap * (key + 4); }
+size_t top_extra(int nt, int cap, size_t key) { return (nt == 32 ? kCountBytes<32> : kCountBytes<kWide>)+16 + (size_t)cap * (key + 4); }
 int top_cap(int k) {  // room for the candidates: a power of two
     int c = 128;
     while (c < 3 * k && c < 2 * HX_READOUT_MAX_K) c *= 2;
@@ -351,7 +402,7 @@ int top_cap(int k) {  // room for the candidates: a power of two
 }
 
 template <typename T, int NT, bool CL>
-__global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ? kBlocks<T> : 6)
+__global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kWide ? kWides<T> : 6)
     top_kernel(const T* __restrict__ xs, int nrow, int ncol, long long ld, int k, Heat heat, int* __restrict__ idx, T* __restrict__ val,
                typename Ty<T>::W* __restrict__ lse, int cap, int team_bytes, int slice_bytes) {
     using W = typename Ty<T>::W;
@@ -417,6 +468,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ?
             if (lead) find_bin(team, hist, k, bin);
             team.sync_all();
             const int b = *team.of(bin, 0);
+            for (int j = t; j < kRanks; j += NT) hist[j] = 0;  // ranks from here on
             gather_bins<T>(team, sl, v0, v1, lane, bag, b, top.mx);
             team.sync_all();
             if (next < nrow) ask(next);
@@ -441,8 +493,10 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ?
                         bag.pos[br.above + at] = i;
                     });
                     n = k;
+                    for (int j = t; j < kRanks; j += NT) hist[j] = 0;
+                    team.sync_block();
                 }
-                in_order(team, bag, n, k, [&](int r, K key, int p) {
+                in_order(team, bag, n, k, (int*)hist, [&](int r, K key, int p) {
                     out_idx[r] = p;
                     out_val[r] = narrow<T>(value_of(key));
                 });
@@ -542,7 +596,7 @@ constexpr int kMassBytes = kRowBins<NT> * 8 > kCountBytes<NT> ? kRowBins<NT> * 8
 static_assert(128 * (8 + 4 + 4 + 4) >= kSlowBytes, "find_border() has the candidates' place");
 size_t sample_extra(int nt, int cap, size_t key) {
     const size_t lists = (size_t)cap * (key + 4) + (size_t)cap * (8 + 4);
-    return nt == 32 ? kMassBytes<32> + 64 + lists : kMassBytes<kBlock> + 64 + lists + (size_t)cap * (key + 4) + kParts * 8;
+    return nt == 32 ? kMassBytes<32> + 64 + lists : kMassBytes<kWide> + 64 + lists + (size_t)cap * (key + 4) + kParts * 8;
 }
 
 // Adds a mass to a bin (two words) in shared memory: the carry goes with the high word.
@@ -565,7 +619,7 @@ __device__ __forceinline__ int past(const u64* cum, int n, u64 target, int lane)
 }
 
 template <typename T, int NT, bool CL>
-__global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ? kBlocks<T> : 6)
+__global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kWide ? kWides<T> : 6)
     sample_kernel(const T* __restrict__ xs, int nrow, int ncol, long long ld, hx_sample_rule rule, const hx_sample_rule* __restrict__ rules,
                   const double* __restrict__ us, int bits, int* __restrict__ idx, typename Ty<T>::W* __restrict__ logp, int cap,
                   int team_bytes, int slice_bytes) {
@@ -664,6 +718,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ?
                 if (lead) find_bin(team, hist, r.top_k, bin);
                 team.sync_all();
                 const int b = *team.of(bin, 0);
+                for (int j = t; j < kRanks; j += NT) hist[j] = 0;  // ranks from here on
                 gather_bins<T>(team, sl, v0, v1, lane, bag, b, top.mx);
                 team.sync_all();
                 if (next < nrow) ask(next);
@@ -687,8 +742,10 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ?
                             bag.pos[br.above + at] = i;
                         });
                         n = r.top_k;
+                        for (int j = t; j < kRanks; j += NT) hist[j] = 0;
+                        team.sync_block();
                     }
-                    in_order(team, bag, n, r.top_k, [&](int j, K key, int p) {
+                    in_order(team, bag, n, r.top_k, (int*)hist, [&](int j, K key, int p) {
                         cum[j] = (u64)key;
                         pos[j] = p;
                     });
@@ -800,8 +857,8 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ?
                         return s > sc.least && -__double2loint(Scale::rounded(s)) >> kCoarse<NT> == b;
                     };
                     // every readout of the bin lies between these
-                    const double width = (double)(1 << kCoarse<NT>) / sc.c, far = (double)(b + 1) * width;
-                    const W hi = (W)(sc.m - ((double)b - 1.0) * width), lo = (W)(sc.m - far);
+                    const double width = (double)(1 << kCoarse<NT>) / sc.c, half = 0.5 / (1 << kCoarse<NT>);
+                    const W hi = (W)(sc.m - ((double)b - 1.001 * half) * width), lo = (W)(sc.m - ((double)(b + 1) - 0.999 * half) * width);
                     gather<T>(team, sl, v0, v1, lane, bag,
                               [&](const Vec<T>& xv) {
                                   bool some = false;
@@ -809,7 +866,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ?
                                   for (int q = 0; q < Ty<T>::VEC; q++) some |= (wide(xv.e[q]) <= hi) & (wide(xv.e[q]) >= lo);
                                   return some;
                               },
-                              in);
+                              [&](W y) { return NW > 1 ? (y <= hi) & (y >= lo) : in(y); });  // a block sorts out the few too many below
                     team.sync_all();
                     if (last && next < nrow) ask(next);
                     if (lead) {
@@ -818,15 +875,17 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ?
                         Bag<K> list = bag;
                         team.sync_block();
                         if constexpr (NW > 1) {
-                            if (n > 64 && n <= cap) {  // by the fraction of the argument: one of kParts parts of the bin
+                            if (n <= cap) {  // by the fraction of the argument: one of kParts parts of the bin
                                 const auto part_of = [&](double v) {
-                                    const double s = sc.arg(v);
-                                    return min(max((int)((0.5 - (s - (Scale::rounded(s) - 6755399441055744.0))) * kParts), 0), kParts - 1);
+                                    const double s = sc.arg(v), y = Scale::rounded(s);
+                                    if (!(s > sc.least) || -__double2loint(y) != b) return -1;
+                                    return min(max((int)((0.5 - (s - (y - 6755399441055744.0))) * kParts), 0), kParts - 1);
                                 };
                                 const unsigned parts_at = (unsigned)__cvta_generic_to_shared(parts);
                                 for (int j = t; j < n; j += NT) {
                                     const double v = (double)value_of(bag.key[j]);
-                                    add_mass(parts_at + part_of(v) * 8, sc.mass(v));
+                                    const int p = part_of(v);
+                                    if (p >= 0) add_mass(parts_at + p * 8, sc.mass(v));
                                 }
                                 team.sync_block();
                                 if (t < 32) {
@@ -872,7 +931,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kBlock ?
                             at.through = br.above + (nth + 1) * m;
                             at.pos = *choice;
                         } else {
-                            in_order(team, list, n, n, [&](int j, K key, int p) {
+                            in_order(team, list, n, n, nullptr, [&](int j, K key, int p) {
                                 cum[j] = (u64)key;
                                 pos[j] = p;
                             });
@@ -970,14 +1029,14 @@ cudaError_t launch_top(const hx_readout& rows, int k, const Heat& heat, int* idx
         const int cap = top_cap(k);
         const size_t key = sizeof(typename Ty<T>::K);
         const bool warps = rows.ncol <= 512 && cap <= 512;
-        const size_t ex = top_extra(warps ? 32 : kBlock, cap, key);
-        const Deal d = deal<T>(rows, ex, warps ? ex : 0, 0, sms);
+        const size_t ex = top_extra(warps ? 32 : kWide, cap, key);
+        const Deal d = deal<T>(rows, ex, warps ? ex : 0, kWide, kWides<T>, 0, sms);
         const auto go = [&](auto* kernel) {
             return launch(kernel, d, st, (const T*)rows.x, rows.nrow, rows.ncol, rows.ld, k, heat, idx, (T*)val, (typename Ty<T>::W*)lse, cap,
                           (int)d.team, (int)d.slice);
         };
-        return d.nt == 32 ? go(top_kernel<T, 32, false>) : d.parts > 1 ? go(top_kernel<T, kBlock, true>)
-               : d.nt == 128 ? go(top_kernel<T, 128, false>) : go(top_kernel<T, kBlock, false>);
+        return d.nt == 32 ? go(top_kernel<T, 32, false>) : d.parts > 1 ? go(top_kernel<T, kWide, true>)
+               : d.nt == 128 ? go(top_kernel<T, 128, false>) : go(top_kernel<T, kWide, false>);
     });
 }
 
@@ -990,17 +1049,17 @@ cudaError_t launch_sample(const hx_readout& rows, const hx_sample_rule& rule, co
         int cap = rows.ncol <= 512 ? 128 : 512;
         if (!rules)
             while (cap < 1024 && rule.top_k >= 1.0 && 2.0 * rule.top_k > cap &&
-                   kRedBytes + Slice<T>::bytes(rows.ncol, 8) + sample_extra(kBlock, 2 * cap, key) <= kSmemBlock)
+                   kRedBytes + Slice<T>::bytes(rows.ncol, 8) + sample_extra(kWide, 2 * cap, key) <= kSmemBlock)
                 cap *= 2;
         const bool warps = rows.ncol <= 512 && cap <= 256;
-        const size_t ex = sample_extra(warps ? 32 : kBlock, cap, key);
-        const Deal d = deal<T>(rows, ex, warps ? ex : 0, 0, sms);
+        const size_t ex = sample_extra(warps ? 32 : kWide, cap, key);
+        const Deal d = deal<T>(rows, ex, warps ? ex : 0, kWide, kWides<T>, 0, sms);
         const auto go = [&](auto* kernel) {
             return launch(kernel, d, st, (const T*)rows.x, rows.nrow, rows.ncol, rows.ld, rule, rules, u, bits, idx, (typename Ty<T>::W*)logp, cap,
                           (int)d.team, (int)d.slice);
         };
-        return d.nt == 32 ? go(sample_kernel<T, 32, false>) : d.parts > 1 ? go(sample_kernel<T, kBlock, true>)
-               : d.nt == 128 ? go(sample_kernel<T, 128, false>) : go(sample_kernel<T, kBlock, false>);
+        return d.nt == 32 ? go(sample_kernel<T, 32, false>) : d.parts > 1 ? go(sample_kernel<T, kWide, true>)
+               : d.nt == 128 ? go(sample_kernel<T, 128, false>) : go(sample_kernel<T, kWide, false>);
     });
 }
 
