@@ -44,8 +44,11 @@ __device__ __forceinline__ float distance(W top, W x) {  // also where both are 
     return x == top ? 0.0f : (float)(top - x);
 }
 
-__device__ __forceinline__ bool before(u64 ka, int pa, u64 kb, int pb) { return ka > kb || (ka == kb && pa < pb); }
-__device__ __forceinline__ bool before(unsigned ka, int pa, unsigned kb, int pb) { return ka > kb || (ka == kb && pa < pb); }
+// whether one candidate comes before another (without branches)
+__device__ __forceinline__ bool before(u64 ka, int pa, u64 kb, int pb) { return (ka > kb) | ((ka == kb) & (pa < pb)); }
+__device__ __forceinline__ bool before(unsigned ka, int pa, unsigned kb, int pb) {
+    return ((u64)ka << 32 | (unsigned)~pa) > ((u64)kb << 32 | (unsigned)~pb);
+}
 
 __device__ __forceinline__ u64 scan(u64 v, int lane) {  // inclusive, over a warp
 #pragma unroll
@@ -95,7 +98,7 @@ __device__ __forceinline__ Top<typename Ty<T>::W> largest(G& team, const Slice<T
         const Vec<T> x = sl.get(v);
         if constexpr (sizeof(W) == 8) {
             fine &= (x.e[0] == x.e[0]) & (x.e[1] == x.e[1]);
-            mx = larger(larger(mx, x.e[0]), x.e[1]);
+            mx = larger(mx, larger(x.e[0], x.e[1]));  // one step of the dependent chain a vector
         } else {
             mx = larger_nan(mx, of_vector(x));
         }
@@ -139,7 +142,7 @@ __device__ __forceinline__ void count_groups(G& team, const Slice<T>& sl, int v0
     for (int v = v0 + lane; v < v1;) {
         W g = -INFINITY;
         const int end = min(v1, v + 32 * per);
-#pragma unroll 2
+#pragma unroll 4
         for (; v < end; v += 32) {
             const Vec<T> x = sl.get(v);
             f(x);
@@ -191,9 +194,9 @@ __device__ __forceinline__ void gather(G& team, const Slice<T>& sl, int v0, int 
         if (!__any_sync(~0u, marks)) continue;
         int hits = 0;
         for (unsigned m = marks; m; m &= m - 1) {
-            const Vec<T> x = sl.get(first + lane + 32 * (__ffs(m) - 1));
-#pragma unroll
-            for (int u = 0; u < VEC; u++) hits += want(wide(x.e[u]));
+            const T* const x = sl.e + (first + lane + 32 * (__ffs(m) - 1)) * VEC;
+#pragma unroll 2
+            for (int u = 0; u < VEC; u++) hits += want(wide(x[u]));
         }
         int upto = hits;
 #pragma unroll
@@ -206,10 +209,10 @@ __device__ __forceinline__ void gather(G& team, const Slice<T>& sl, int v0, int 
         p = __shfl_sync(~0u, p, 31) + upto - hits;
         for (unsigned m = hits ? marks : 0u; m; m &= m - 1) {
             const int v = first + lane + 32 * (__ffs(m) - 1);
-            const Vec<T> x = sl.get(v);
-#pragma unroll
+            const T* const x = sl.e + v * VEC;
+#pragma unroll 1
             for (int u = 0; u < VEC; u++) {
-                const auto y = wide(x.e[u]);
+                const auto y = wide(x[u]);
                 if (want(y)) {
                     if (p < bag.cap) {
                         key[p] = key_of(y);
@@ -230,7 +233,10 @@ __device__ __forceinline__ void gather_bins(G& team, const Slice<T>& sl, int v0,
     const W lowest = sizeof(W) == 8 ? (W)-1.7976931348623157e308 : (W)-3.4028234663852886e38f;
     if (b >= kBins<G::NT> - 1 || !(least > lowest)) least = lowest;
     if (top == (W)INFINITY && b < kBins<G::NT> - 1) least = top;
-    gather<T>(team, sl, v0, v1, lane, bag, [&](const Vec<T>& x) { return !(of_vector(x) < least); }, [&](W y) { return y >= least; });
+    gather<T>(team, sl, v0, v1, lane, bag, [&](const Vec<T>& x) {
+        if constexpr (sizeof(W) == 8) return (bool)((x.e[0] >= least) | (x.e[1] >= least));
+        return of_vector(x) >= least;
+    }, [&](W y) { return y >= least; });
 }
 
 // The n candidates in order: put(rank, key, position) for the first `want`, by
@@ -253,7 +259,7 @@ __device__ __forceinline__ void in_order(G& team, const Bag<K>& bag, int n, int 
             if (j < n) {
                 k = bag.key[j];
                 p = bag.pos[j];
-#pragma unroll 4
+#pragma unroll 8
                 for (int l = l0; l < l1; l++) r += before(bag.key[l], bag.pos[l], k, p);
                 if (r) atomicAdd(ranks + j, r);
             }
