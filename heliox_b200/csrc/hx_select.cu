@@ -118,6 +118,13 @@ __device__ __forceinline__ Top<typename Ty<T>::W> largest(G& team, const Slice<T
 // distance from the largest; what is as near as the bin that the k-th falls
 // into is gathered.
 
+// Measured (B200): 4000 x 10000 fp64, k 64, with log-sum-exp: 155 us (2.1 TB/s;
+// 74 candidates a row); 1024 x 32000 fp16, k 100: 45 us; 8001 x 302 fp64, a warp
+// a row: 28 us.  Bound by the latency of the passes over shared memory, with two
+// to three rows an SM.  Bins of an eighth of an octave let in more candidates
+// than the list holds where a few readouts stand far above the others (5000
+// columns: 189 us for 1184 rows, 55 with a thirty-second).
+
 // Each lane's vectors in groups; each group's maximum is counted in the
 // leading block's histogram.  f(vector) sees every vector.
 template <typename T, typename G, typename F>
@@ -400,7 +407,7 @@ __device__ void first_of_key(G& team, const T* __restrict__ x, int n, u64 key, u
 
 template <int NT>
 constexpr int kCountBytes = kBins<NT> * 4 > kSlowBytes ? kBins<NT> * 4 : kSlowBytes;
-size_t top_extra(int nt, int cap, size_t key) { return (nt == 32 ? kCountBytes<32> : kCountBytes<kWide>)+16 + (size_t)cap * (key + 4); }
+size_t top_extra(int nt, int cap, size_t key) { return (nt == 32 ? kCountBytes<32> : kCountBytes<kWide>) + 16 + (size_t)cap * (key + 4); }
 int top_cap(int k) {  // room for the candidates: a power of two
     int c = 128;
     while (c < 3 * k && c < 2 * HX_READOUT_MAX_K) c *= 2;
@@ -533,6 +540,11 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kWide ? 
 // min_p each keep a first run, so that the shortest of the three is known by
 // its mass, and the choice is the first readout whose running mass exceeds
 // u times that.
+//
+// Measured (B200): 2000 x 10000 fp64, top_p: 140 us (two gathers; one without
+// top_p); 64 x 32000 fp32 with rules of their own: 13 us, a row two blocks;
+// 8001 x 302 fp64, a warp a row: 33 us.  Ranking a whole bin's candidates (208
+// of 10000 columns) instead of one of its 128 parts took 225 us.
 //
 // With top_k the candidates are the k largest, in order.  Without it the
 // masses are summed up in bins of a sixteenth of an octave (the whole part of
