@@ -537,9 +537,10 @@ int hx_mse_loss_grad_noalloc(const double* trace_dev, const double* target_dev, 
  * that the teacher may be another model (fp32, fp16 or bf16 logits).
  * Pointers inside the descriptors are device pointers on the context's device.
  * The work is enqueued on the context's stream; the entries allocate nothing,
- * keep no state between calls and may be captured into CUDA graphs.  Results
- * do not depend on how the work is split or timed: two calls on the same
- * inputs give the same bits.  A -inf readout is a closed choice: it has
+ * keep no state between calls and may be captured into CUDA graphs.  Two calls
+ * with the same arguments give the same bits; positions and choices are also the
+ * same however rows are batched and aligned (sums of floats may then add up in
+ * another order).  A -inf readout is a closed choice: it has
  * probability 0 and is never taken.  "Statistics" (log-sum-exp, losses,
  * log-probabilities) are double for HX_DT_F64 rows and float for the others.
  * The reference has no counterpart (its objectives are Python callables on the

@@ -664,6 +664,77 @@ def test_long_rows_of_equal_readouts(sim, dtype, nrow):
     check_distill(sim, x, order, val, lse, 1.0, dtype, "f64", scale=10.0)
 
 
+@pytest.mark.parametrize("dtype,nrow,ncol,k", [("f64", 2000, 700, 200), ("bf16", 2000, 700, 200), ("f64", 700, 2500, 130), ("f32", 700, 2500, 130),
+                                               ("f64", 80, 60001, 300), ("f16", 90, 300007, 40), ("f64", 9000, 33, 40)])
+def test_more_rows_than_the_card_holds_at_once(sim, dtype, nrow, ncol, k):
+    # teams take several rows in turn: rows without weight, without slots, with NaN and closed ones among them, in every order
+    rng = np.random.default_rng(nrow + ncol)
+    x = readouts(rng, nrow, ncol, dtype)
+    kind = rng.integers(0, 8, nrow)
+    x[kind == 1, 0] = np.nan
+    x[kind == 2] = -np.inf
+    check_top(sim, x, min(k, ncol), 1.0, dtype)
+    check_sample(sim, x, rng.random(nrow), dtype, temperature=1.3, top_p=0.9)
+    rules = np.stack([0.5 + rng.random(nrow), rng.integers(0, 2 * k, nrow) * (rng.random(nrow) < 0.6), 0.3 + 0.6 * rng.random(nrow),
+                      0.1 * rng.random(nrow) * (rng.random(nrow) < 0.5)], 1)
+    check_sample(sim, x, rng.random(nrow), dtype, rules=rules)
+    order, val, lse = teacher(rng, np.where(np.isfinite(x), x, 0.0), k, 1.0, True)
+    order[kind == 3] = -1
+    w = np.where((kind == 4) | (kind == 5), 0.0, 1.0)
+    for rest in (False, True):
+        check_distill(sim, x, order, val, lse if rest else None, 1.0, dtype, dtype, w=w, scale=1.0)
+
+
+def test_offsets_beyond_32_bits(sim):
+    ncol, ld = 1001, 2**31 + 24
+    a = readouts(np.random.default_rng(3), 2, ncol, "f16")
+    buf = torch.empty(ld + ncol, dtype=torch.float16, device="cuda")
+    view = buf.as_strided((2, ncol), (ld, 1))
+    view.copy_(torch.from_numpy(a).half())
+    xx = wide(view)
+    idx, val, lse = call_top(sim, view, ld, 5, 1.0, "f16")
+    for r in range(2):
+        i, v, l = plain_top(xx[r], 5, 1.0)
+        assert np.array_equal(idx[r], i) and np.array_equal(val[r], v)
+    c, lp = call_sample(sim, view, ld, [0.3, 0.8], "f16")
+    assert all(c[r] in plain_sample(xx[r], 1.0, 0, 1.0, 0.0, [0.3, 0.8][r])[2] for r in range(2))
+    rec = record(idx, val, lse, "f32")
+    # rows of the same alignment: another one may add a row's terms up in another order
+    near, near_view, near_ld = place(a, "f16", pad=7)
+    assert torch.equal(near_view, view) and near_ld * 2 % 16 == ld * 2 % 16 == 0
+    want, rl, lo = call_distill(sim, near_view, near_ld, rec, 1.0, "f16", "f32")
+    got, rl2, lo2 = call_distill(sim, view, ld, rec, 1.0, "f16", "f32", in_place=True)
+    assert torch.equal(got, want) and np.array_equal(rl, rl2) and lo == lo2
+
+
+def test_two_contexts_at_once():
+    # calls of two contexts on streams of their own, from two threads
+    import threading
+
+    from heliox_b200.runtime import Sim
+
+    rng = np.random.default_rng(4)
+    want, got, sims = [], [None, None], []
+    data = [readouts(rng, 60, 9001, "f64") for _ in range(2)]
+    for j in range(2):
+        s = Sim(0)
+        s.set_stream(torch.cuda.Stream().cuda_stream)
+        sims.append(s)
+        buf, view, ld = place(data[j], "f64")
+        want.append((view, call_top(s, view, ld, 20, 1.0, "f64")))
+
+    def work(j):
+        for _ in range(5):
+            got[j] = call_top(sims[j], want[j][0], 9001, 20, 1.0, "f64")
+
+    ts = [threading.Thread(target=work, args=(j,)) for j in range(2)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    for j in range(2):
+        assert all(np.array_equal(a, b) for a, b in zip(got[j], want[j][1]))
+        sims[j].close()
+
+
 def test_same_bits_twice_and_whatever_the_batch(sim):
     rng = np.random.default_rng(2)
     for dtype, n in (("f64", 302), ("f64", 9001), ("bf16", 30011), ("f32", 120)):
