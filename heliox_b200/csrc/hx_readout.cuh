@@ -13,6 +13,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cmath>
 #include <cstdio>
@@ -447,9 +448,14 @@ cudaError_t launch(void (*kernel)(P...), const Deal& d, cudaStream_t st, A... ar
     return cudaLaunchKernelEx(&c, kernel, P(args)...);
 }
 
-inline int sm_count(int device) {
-    int n = 0;
-    return cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) == cudaSuccess ? n : 1;
+inline int sm_count(int device) {  // asked once a device
+    static std::atomic<int> known[64];
+    std::atomic<int>* const k = device >= 0 && device < 64 ? known + device : nullptr;
+    int n = k ? k->load(std::memory_order_relaxed) : 0;
+    if (n > 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 1;
+    if (k) k->store(n, std::memory_order_relaxed);
+    return n;
 }
 
 template <typename F>

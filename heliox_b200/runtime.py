@@ -387,8 +387,8 @@ class Sim:
         (float64 for "f64" rows, else float32), 0 to leave them out."""
         rows = _readout(logits_ptr, nrow, ncol, dtype, ld)
         self._check(self._L.hx_top_logits_dev(self._ctx, C.byref(rows), int(k), float(temperature),
-                                              C.c_void_p(int(idx_ptr)), C.c_void_p(int(val_ptr)),
-                                              C.c_void_p(int(lse_ptr))), "hx_top_logits_dev")
+                                              int(idx_ptr), int(val_ptr),
+                                              int(lse_ptr)), "hx_top_logits_dev")
 
     def distill_loss_grad_dev(self, logits_ptr: int, nrow: int, ncol: int, k: int, t_idx_ptr: int, t_val_ptr: int,
                               grad_ptr: int, row_loss_ptr: int, loss_ptr: int, *, t_lse_ptr: int = 0,
@@ -408,9 +408,9 @@ class Sim:
         t = _lib.Teacher(int(t_idx_ptr), int(t_val_ptr), int(t_lse_ptr) or None, _dt(t_dtype or dtype), int(k))
         sc = (1.0 / nrow if nrow > 0 else 1.0) if scale is None else float(scale)
         self._check(self._L.hx_distill_loss_grad_dev(
-            self._ctx, C.byref(rows), C.byref(t), float(temperature), sc, C.c_void_p(int(row_weight_ptr)),
-            C.c_void_p(int(grad_ptr)), int(ncol if ld_grad is None else ld_grad), C.c_void_p(int(row_loss_ptr)),
-            C.c_void_p(int(loss_ptr))), "hx_distill_loss_grad_dev")
+            self._ctx, C.byref(rows), C.byref(t), float(temperature), sc, int(row_weight_ptr),
+            int(grad_ptr), int(ncol if ld_grad is None else ld_grad), int(row_loss_ptr),
+            int(loss_ptr)), "hx_distill_loss_grad_dev")
 
     def sample_dev(self, logits_ptr: int, nrow: int, ncol: int, u_ptr: int, idx_ptr: int, *, logp_ptr: int = 0,
                    temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
@@ -424,9 +424,9 @@ class Sim:
         top_p, min_p of each row) in place of the four arguments."""
         rows = _readout(logits_ptr, nrow, ncol, dtype, ld)
         rule = _lib.SampleRule(float(temperature), float(top_k), float(top_p), float(min_p))
-        self._check(self._L.hx_sample_dev(self._ctx, C.byref(rows), C.byref(rule), C.c_void_p(int(rules_ptr)),
-                                          C.c_void_p(int(u_ptr)), C.c_void_p(int(idx_ptr)),
-                                          C.c_void_p(int(logp_ptr))), "hx_sample_dev")
+        self._check(self._L.hx_sample_dev(self._ctx, C.byref(rows), C.byref(rule), int(rules_ptr),
+                                          int(u_ptr), int(idx_ptr),
+                                          int(logp_ptr)), "hx_sample_dev")
 
     # ------------------------------------------------------------------ optimizer
     # Mirrors Sim.create_optimizer / configure_optimizer / optimizer_add_external_grads /
