@@ -150,8 +150,8 @@ struct Slots {
         double ref = 0;
         if (lanes) {
             int j = __ffs(lanes) - 1;
-            while (at[j] < 0) j += 32;  // that lane's first slot in use
-            ref = (double)wide(row[at[j]]);
+            while (j < k && at[j] < 0) j += 32;  // that lane's first slot in use
+            if (j < k) ref = (double)wide(row[at[j]]);
         }
         if (!te.lse) {
 #pragma unroll
@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT + 32, NT == kBl
     char* const mine = smem + (ONE ? (threadIdx.x >> 5) * team_bytes : 0);
     Team<NT, CL, !ONE> team(mine);
     const int t = team.t, k = te.k;
-    const bool few = k <= kFewSlots;
+    const bool few = ONE || k <= kFewSlots;  // a warp's record is copied ahead of its row: deal() gives warps no more slots
     const bool helper = ONE || t >= NT, worker = ONE || t < NT;
     T* const row_mem = (T*)(mine + kRedBytes);
     char* const lists = mine + kRedBytes + slice_bytes;
@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT + 32, NT == kBl
             if (ONE) commit_copies();  // the row's; the slots' are the group before
         }
         if (helper && wn != 0.0) {
-            if (!few) ahead.load(te, next);
+            if (!few) ahead.load(te, next);  // by a helper, which has no copies besides
             if (ONE || !few || !live) ahead.template sift<ONE ? 1 : 0>(te, xs + next * ld, ncol, hash);
             ahead.weigh(te, heat.inv);
         }
@@ -571,7 +571,8 @@ int hx_distill_loss_grad_dev(hx_ctx* ctx, const hx_readout* rows, const hx_teach
         using T = std::remove_pointer_t<decltype(t)>;
         using W = typename Ty<T>::W;
         if (rows->nrow > 0) {
-            const Deal d = deal<T>(*rows, distill_extra(teacher->k), distill_extra(kFewSlots), kBlock, kBlocks<T>, 32, sm_count(ctx->device));
+            const size_t extra = distill_extra(teacher->k);
+            const Deal d = deal<T>(*rows, extra, teacher->k <= kFewSlots ? extra : 0, kBlock, kBlocks<T>, 32, sm_count(ctx->device));
             auto go = [&](auto* kernel) {
                 return launch(kernel, d, ctx->st, (const T*)rows->x, rows->nrow, rows->ncol, rows->ld, *teacher, heat_of(temperature),
                               scale, row_weight_dev, (T*)grad_dev, ld_grad, (W*)row_loss_dev, (int)d.team, (int)d.slice);

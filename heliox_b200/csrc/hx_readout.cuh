@@ -403,7 +403,8 @@ struct Deal {
 };
 constexpr size_t kSmemBlock = 227 * 1024, kSmemSM = 228 * 1024;
 
-// Warps take short rows, blocks of 128 and 256 threads longer ones.  A row
+// Warps take short rows (where what they need besides is at most warp_extra
+// bytes), blocks of 128 and 256 threads longer ones.  A row
 // that no block can hold is shared by a cluster of blocks, and one of few rows
 // too, so that the card is not left idle.
 template <typename T>

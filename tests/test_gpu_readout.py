@@ -822,3 +822,20 @@ def test_refusals_leave_the_context_usable(sim):
     with pytest.raises(HxError, match="top_p"):
         sim.sample_dev(x.data_ptr(), 2, 4, x.data_ptr(), i.data_ptr(), top_p=1.5)
     check_top(sim, np.eye(4), 2, 1.0, "f64")
+
+
+@pytest.mark.parametrize("ncol,k,dtype,t_dtype,rest", [(302, 129, "f64", "f64", True), (302, 150, "f64", "f32", False), (302, 204, "f64", "bf16", True),
+                                                       (302, 205, "f64", "f64", False), (512, 128, "f64", "f64", True), (512, 129, "f32", "f32", True),
+                                                       (512, 150, "bf16", "bf16", False), (512, 204, "f64", "f32", True), (512, 205, "f16", "f64", True)])
+def test_distill_many_slots_on_many_short_rows(sim, ncol, k, dtype, t_dtype, rest):
+    # each team takes several rows, whose records differ: dropped and doubled positions, other ones in every row
+    rng = np.random.default_rng(ncol * 1000 + k)
+    nrow = 8000
+    x = readouts(rng, nrow, ncol, dtype)
+    order, val, lse = teacher(rng, x, k, 2.0, rest)
+    mix = rng.permuted(np.tile(np.arange(k), (nrow, 1)), axis=1)
+    order, val = np.take_along_axis(order, mix, 1), np.take_along_axis(val, mix, 1)
+    r = np.arange(nrow)
+    order[r, rng.integers(0, k, nrow)] = order[r, rng.integers(0, k, nrow)]
+    order[rng.random(order.shape) < 0.1] = -1
+    check_distill(sim, x, order, val, lse, 2.0, dtype, t_dtype, scale=1.0)
