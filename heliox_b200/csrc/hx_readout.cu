@@ -295,6 +295,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT + 32, NT == kBl
                         __syncwarp();
                         ask(sl);
                         wait_copies();
+                        __syncwarp();
                         for (int v = v0 + lane; v < v1; v += 32) {
                             const Vec<T> x = sl.get(v);
 #pragma unroll

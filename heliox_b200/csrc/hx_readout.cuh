@@ -260,7 +260,8 @@ struct Team {
     }
 };
 
-// Asynchronous copies into shared memory; wait_copies() waits for the thread's own.
+// Asynchronous copies into shared memory; wait_copies() waits for the thread's
+// own: a barrier of the warp follows it before other lanes' copies are read.
 __device__ __forceinline__ void copy8(void* d, const void* g) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((unsigned)__cvta_generic_to_shared(d)), "l"(g) : "memory");
 }
@@ -374,6 +375,7 @@ struct Slice {
                     if (i >= 0 && i < n) dst[i] = x.e[u];
                 }
             }
+            __syncwarp();  // every lane has read its vectors
         }
     }
 };

@@ -455,8 +455,8 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kWide ? 
             *bin = kBins<NT> - 1;
         }
         wait_copies();
+        __syncwarp();  // the lanes' copies are the warp's from here on
         if (next < nrow) prefetch(next);
-        if (NT == 32) __syncwarp();
         const Top<W> top = largest<T>(team, sl, v0, v1, lane);
         if (NT == 32) __syncwarp();
         int* const out_idx = idx + row * k;
@@ -692,8 +692,8 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT, NT == kWide ? 
             *bin = kBins<NT> - 1;
         }
         wait_copies();
+        __syncwarp();  // the lanes' copies are the warp's from here on
         if (next < nrow) prefetch(next);
-        if (NT == 32) __syncwarp();
         const Top<W> top = largest<T>(team, sl, v0, v1, lane);
         if (NT == 32) __syncwarp();
         const bool odd = top.odd || given.temperature != given.temperature;

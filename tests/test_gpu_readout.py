@@ -839,3 +839,20 @@ def test_distill_many_slots_on_many_short_rows(sim, ncol, k, dtype, t_dtype, res
     order[r, rng.integers(0, k, nrow)] = order[r, rng.integers(0, k, nrow)]
     order[rng.random(order.shape) < 0.1] = -1
     check_distill(sim, x, order, val, lse, 2.0, dtype, t_dtype, scale=1.0)
+
+
+@pytest.mark.parametrize("dtype,nrow,ncol", [("f64", 700, 2051), ("f32", 1200, 2053), ("bf16", 1200, 4099), ("f16", 1300, 611), ("f64", 40, 20001), ("f64", 5000, 37)])
+def test_edges_of_unaligned_rows(sim, dtype, nrow, ncol):
+    # rows that start inside a vector, NaN between them: the largest readouts stand at the row's ends, which lanes copy for one another
+    rng = np.random.default_rng(nrow + ncol)
+    x = readouts(rng, nrow, ncol, dtype)
+    at = np.where(rng.random(nrow) < 0.5, rng.integers(0, 9, nrow), ncol - 1 - rng.integers(0, 9, nrow))
+    r = np.arange(nrow)
+    x[r, at] = (-65.0 if dtype == "f64" else 0.0) + 60.0 + rng.integers(0, 30, nrow)
+    for pad, offset in ((1, 1), (3, 0)):
+        check_top(sim, x, 5, 1.0, dtype, pad, offset)
+        assert np.array_equal(check_sample(sim, x, rng.random(nrow), dtype, pad, offset, top_k=3), at)
+        assert np.array_equal(check_sample(sim, x, rng.random(nrow), dtype, pad, offset), at)
+        # the slots' readouts are the smallest: the loss reads the row again and seeks its largest
+        order = np.argsort(x, axis=1, kind="stable")[:, :4]
+        check_distill(sim, x, order, rng.standard_normal(order.shape), None, 0.25, dtype, "f64", scale=4.0, pad=pad, offset=offset, grad_ld=ncol + 2)
