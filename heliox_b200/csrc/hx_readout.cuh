@@ -435,8 +435,9 @@ template <typename... P, typename... A>
 cudaError_t launch(void (*kernel)(P...), const Deal& d, cudaStream_t st, A... args) {
     cudaLaunchConfig_t c{};
     c.dynamicSmemBytes = d.nt == 32 ? d.team * kWarpRows : d.team;
+    // the limit is the kernel's, for every thread and context: always the same one, so that no call takes it from another
     if (c.dynamicSmemBytes > 48 * 1024)
-        if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)c.dynamicSmemBytes)) return e;
+        if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBlock)) return e;
     c.gridDim = dim3((unsigned)d.blocks);
     c.blockDim = dim3(d.nt == 32 ? 32 * kWarpRows : d.nt + d.help);
     c.stream = st;

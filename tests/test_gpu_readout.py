@@ -856,3 +856,60 @@ def test_edges_of_unaligned_rows(sim, dtype, nrow, ncol):
         # the slots' readouts are the smallest: the loss reads the row again and seeks its largest
         order = np.argsort(x, axis=1, kind="stable")[:, :4]
         check_distill(sim, x, order, rng.standard_normal(order.shape), None, 0.25, dtype, "f64", scale=4.0, pad=pad, offset=offset, grad_ld=ncol + 2)
+
+
+def test_two_threads_with_rows_of_other_lengths():
+    # the same kernel with more and with less shared memory, from two threads that call without a pause
+    import ctypes as C
+    import os
+    import subprocess
+
+    from heliox_b200 import _lib
+    from heliox_b200.runtime import Sim
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = os.path.join(root, "tests", "capi", "_build")
+    os.makedirs(out, exist_ok=True)
+    so = os.path.join(out, "two_threads.so")
+    subprocess.run(["g++", "-std=c++17", "-O2", "-shared", "-fPIC", "-I" + os.path.join(root, "include"),
+                    os.path.join(root, "tests", "capi", "two_threads.cpp"), "-o", so, "-L" + os.path.join(root, "heliox_b200"), "-lhx_b200",
+                    "-Wl,-rpath," + os.path.join(root, "heliox_b200"), "-pthread"], check=True)
+    nrow, k, rng = 2, 8, np.random.default_rng(6)
+    sims, views, idx, val = [], [], [], []
+    for n in (60000, 45000):
+        sims.append(Sim(0))
+        views.append(place(rng.standard_normal((nrow, n)), "f64")[1])
+        idx.append(torch.empty((nrow, k), dtype=torch.int32, device="cuda"))
+        val.append(torch.empty((nrow, k), dtype=torch.float64, device="cuda"))
+    torch.cuda.synchronize()
+    two = C.CDLL(so).two_threads
+    two.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int]
+    ptrs = [(C.c_void_p * 2)(*a) for a in ([s._ctx for s in sims], [t.data_ptr() for t in idx], [t.data_ptr() for t in val])]
+    rows = (_lib.Readout * 2)(*[_lib.Readout(v.data_ptr(), 0, nrow, v.shape[1], v.shape[1]) for v in views])
+    assert two(ptrs[0], rows, k, ptrs[1], ptrs[2], 20000) == 0
+    torch.cuda.synchronize()
+    for j in range(2):
+        assert np.array_equal(idx[j].cpu().numpy(), np.argsort(-wide(views[j]), axis=1, kind="stable")[:, :k])
+        sims[j].close()
+
+
+def test_calls_of_other_lengths_in_one_graph(sim):
+    # a long row's call keeps its shared memory when shorter rows follow, in a graph that is put together after both
+    from heliox_b200.runtime import Sim
+
+    rng = np.random.default_rng(7)
+    s, st = Sim(0), torch.cuda.Stream()
+    parts = []
+    for n in (20001, 7001, 9001):
+        buf, view, ld = place(rng.standard_normal((150, n)), "f64")
+        parts.append((n, view, torch.empty((150, 4), dtype=torch.int32, device="cuda"), torch.empty((150, 4), dtype=torch.float64, device="cuda")))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        s.set_stream(st.cuda_stream)
+        for n, view, i, v in parts:
+            s.top_logits_dev(view.data_ptr(), 150, n, 4, i.data_ptr(), v.data_ptr())
+    graph.replay()
+    torch.cuda.synchronize()
+    for n, view, i, v in parts:
+        assert np.array_equal(i.cpu().numpy(), np.argsort(-wide(view), axis=1, kind="stable")[:, :4])
+    s.close()
