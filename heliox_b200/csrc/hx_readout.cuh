@@ -93,8 +93,8 @@ __device__ __forceinline__ double load_any(const void* p, int dtype, size_t i) {
 // 16 k + j puts the power of two in.  11 fp64 operations and one table entry:
 // 16 doubles are one entry per pair of shared-memory banks, so lanes never
 // wait for one another; 64 entries would save two operations and cost four
-// more conflicts.  Below 2^-1022 it is 0; above 2^1000 (and for NaN) it is
-// about 2^1000, which the caller sees in the sum.
+// more conflicts.  Below 2^-1018 it is 0; above 2^1000 it is about 2^1000, for
+// NaN that (sign bit clear) or NaN, which the caller sees in the sum.
 // fp32: the hardware's 2^x (about 3 half steps); results below 2^-126 are 0.
 constexpr int kPowBytes = 16 * 8;
 __constant__ unsigned long long kPow16[16] = {
@@ -104,16 +104,16 @@ __constant__ unsigned long long kPow16[16] = {
 struct Heat {  // a temperature, worked out on the host
     double t, inv, c;  // c = 16 log2(e) / T
     int high;          // high word of the largest d that is taken as it is
-    unsigned low;      // and of the d below which the result is 0
+    unsigned low, span;  // and of the d below which the result is 0; from there to -inf's, NaN's being beyond
     float cf;          // log2(e) / T
 };
 struct Scaler64 {
     double c, m, inv;
     int high;
-    unsigned low;
+    unsigned low, span;
     const int2* pow16;  // kPow16 in shared memory
     __device__ __forceinline__ Scaler64(const Heat& h, double m_, const char* table)
-        : c(h.c), m(m_), inv(h.inv), high(h.high), low(h.low), pow16((const int2*)table) {}
+        : c(h.c), m(m_), inv(h.inv), high(h.high), low(h.low), span(h.span), pow16((const int2*)table) {}
     __device__ __forceinline__ double operator()(double x) const {
         const double d0 = x - m;
         const double d = __hiloint2double(min(__double2hiint(d0), high), __double2loint(d0));
@@ -130,7 +130,7 @@ struct Scaler64 {
         const int2 t = pow16[k & 15];
         const double p = __hiloint2double(t.y + (k << 16), t.x);
         const double e = __fma_rn(p, q, p);
-        return (unsigned)__double2hiint(d) > low ? 0.0 : e;
+        return (unsigned)__double2hiint(d) - low <= span ? 0.0 : e;
     }
     __device__ __forceinline__ double z(double x) const { return (x - m) * inv; }  // of which it is the exponential
     static constexpr double most = 0x1p500;  // a sum up to here has left no readout out
@@ -394,7 +394,8 @@ inline Heat heat_of(double t) {
         return (unsigned)(b >> 32);
     };
     h.high = (int)high_word(16000.0 / h.c);
-    h.low = high_word(-16300.0 / h.c);
+    h.low = high_word(-16300.0 / h.c) + 1;
+    h.span = 0xfff00000u - h.low;
     return h;
 }
 

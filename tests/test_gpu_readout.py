@@ -913,3 +913,28 @@ def test_calls_of_other_lengths_in_one_graph(sim):
     for n, view, i, v in parts:
         assert np.array_equal(i.cpu().numpy(), np.argsort(-wide(view), axis=1, kind="stable")[:, :4])
     s.close()
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_nan_of_either_sign(sim, dtype):
+    # a NaN outside the slots, with its sign bit set (as the host's and the device's invalid operations make it) and clear
+    bits = {"f64": (0xFFF8 << 48, torch.int64, 64), "f32": (0xFFC0 << 16, torch.int32, 32), "f16": (0xFE00, torch.int16, 16), "bf16": (0xFFC0, torch.int16, 16)}
+    word, itype, size = bits[dtype]
+    rng = np.random.default_rng(11)
+    for nrow, n in ((3, 40), (3, 700), (200, 9000), (3, 60001)):
+        x = readouts(rng, nrow, n, dtype)
+        order, val, lse = teacher(rng, x, 6, 1.0, True)
+        free = [next(i for i in range(n - 1, 0, -1) if i not in order[r]) for r in (0, 1)]
+        buf, view, ld = place(x, dtype)
+        view.view(itype)[0, free[0]] = word - (1 << size)
+        view.view(itype)[1, free[1]] = word - (1 << (size - 1))
+        xx = wide(view)
+        assert np.isnan(xx[0, free[0]]) and np.isnan(xx[1, free[1]])
+        idx, v, ls = call_top(sim, view, ld, 6, 1.0, dtype)
+        assert (idx[:2] == -1).all() and np.isnan(v[:2]).all() and np.isnan(ls[:2]).all() and (idx[2:] >= 0).all()
+        c, lp = call_sample(sim, view, ld, rng.random(nrow), dtype)
+        assert (c[:2] == -2).all() and np.isnan(lp[:2]).all() and (c[2:] >= 0).all()
+        for rest in (False, True):
+            g, rl, lo = call_distill(sim, view, ld, record(order, val, lse if rest else None, "f64"), 1.0, dtype, "f64")
+            assert np.isnan(rl[:2]).all() and np.isnan(wide(g[:2])).all() and math.isnan(lo)
+            assert np.isfinite(rl[2:]).all() and torch.isfinite(g[2:]).all()
