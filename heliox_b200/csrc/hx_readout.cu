@@ -28,7 +28,9 @@ using namespace hxr;
 //
 // The slots' readouts are lifted out of the row before the sum (-inf stands in
 // their places), so that the sum over the rest is a sum of its own and not a
-// difference.  The teacher's side of the next row is worked out meanwhile: in
+// difference.  A rest that the record gives a share, but that lies e^-44 or more
+// below, is summed up again relative to its own largest readout, so that its
+// logarithm and its readouts' shares of it are right at any distance.  The teacher's side of the next row is worked out meanwhile: in
 // a block of many warps by a helper, which has no run, so that its chain of
 // dependent exponentials and reductions is waited for by nobody.
 
@@ -43,6 +45,7 @@ constexpr int kBlocks = sizeof(T) == 8 ? 2 : 3;  // such blocks on an SM, where 
 // Blocks of 512 threads: 199 us for the first, 62 for the second (each warp has
 // its share of reductions and divisions once a row); 3 blocks of 256 an SM
 // against 2: 50 and 55 us for the second.
+constexpr double kFar = 0x1p-64;  // a sum from here on has lost no readout that counts to the exponentials' range (2^-126 in fp32)
 constexpr int kFewSlots = 128;  // up to here the next row's slots are worked out into lists of their own
 
 __host__ __device__ constexpr int slot_list(int k) { return (k + 3) / 4 * 4; }
@@ -283,6 +286,24 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT + 32, NT == kBl
             struct Sums {
                 double out, in, qz;
             } s;
+            // the exponentials of this warp's run, in the readouts' place where they fit, and the lanes' sums
+            const auto sum_up = [&](const auto& ex) {
+                W part[2] = {0, 0};
+#pragma unroll UNROLL
+                for (int v = v0 + lane; v < v1; v += 32) {
+                    Vec<T> x = sl.get(v);
+#pragma unroll
+                    for (int u = 0; u < VEC; u++) {
+                        const W e = ex(wide(x.e[u]));
+                        part[u & 1] += e;
+                        if constexpr (sizeof(T) == sizeof(W)) x.e[u] = e;
+                    }
+                    if constexpr (sizeof(T) == sizeof(W)) sl.set(v, x);
+                }
+                return (double)part[0] + (double)part[1];
+            };
+            const auto add = [](double a, double b) { return a + b; };
+            const auto close = [](int, T* cell) { *cell = narrow<T>((W)-INFINITY); };
             W m = (W)slots.notes[4];
             bool odd = false, empty = false;  // NaN or +inf in the row; no readout is open
             for (bool sure = false;; sure = true) {
@@ -318,30 +339,18 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT + 32, NT == kBl
                 if (worker) {
                     slots.each(sl, k, v0, v1, [&](int j, T* cell) {
                         slots.x[j] = (double)wide(*cell);
-                        *cell = narrow<T>((W)-INFINITY);
+                        close(j, cell);
                     });
                     __syncwarp();
                     if (!ONE) bar_arrive(2, NT + 32);
-                    W part[2] = {0, 0};
-#pragma unroll UNROLL
-                    for (int v = v0 + lane; v < v1; v += 32) {
-                        Vec<T> x = sl.get(v);
-#pragma unroll
-                        for (int u = 0; u < VEC; u++) {
-                            const W e = ex(wide(x.e[u]));
-                            part[u & 1] += e;
-                            if constexpr (sizeof(T) == sizeof(W)) x.e[u] = e;
-                        }
-                        if constexpr (sizeof(T) == sizeof(W)) sl.set(v, x);
-                    }
-                    out = (double)part[0] + (double)part[1];
+                    out = sum_up(ex);
                 }
                 if (helper) {
                     if (!ONE) bar_sync(2, NT + 32);
                     slots.lifted(sl, k, ex);
                     if (!ONE && few && wn != 0.0 && !sure) ahead.template sift<0>(te, xs + next * ld, ncol, hash);
                 }
-                out = team.reduce(out, [](double a, double b) { return a + b; });
+                out = team.reduce(out, add);
                 if (ONE) __syncwarp();
                 s = team.across(Sums{out, slots.notes[5], slots.notes[6]},
                                 [](Sums a, Sums b) { return Sums{a.out + b.out, a.in + b.in, a.qz + b.qz}; });
@@ -350,14 +359,41 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT + 32, NT == kBl
             const double sum_q = slots.notes[1], sum_qlq = slots.notes[2];
             const double total = odd ? (double)NAN : s.in + s.out;
             double qr = te.lse ? (sum_q == sum_q ? larger(0.0, 1.0 - sum_q) : sum_q) : 0.0;
+            // a rest far below: once more, relative to its own largest readout
+            W m_out = m;
+            if (qr > 0.0 && s.out < kFar && !odd && !empty) {
+                W mx = -INFINITY;
+                if (worker) {
+                    if constexpr (sizeof(T) == sizeof(W)) {
+                        __syncwarp();
+                        ask(sl);
+                        wait_copies();
+                        __syncwarp();
+                        slots.each(sl, k, v0, v1, close);
+                        __syncwarp();
+                    }
+                    for (int v = v0 + lane; v < v1; v += 32) {
+                        const Vec<T> x = sl.get(v);
+#pragma unroll
+                        for (int u = 0; u < VEC; u++) mx = larger(mx, wide(x.e[u]));
+                    }
+                }
+                const auto op = [](W a, W b) { return larger(a, b); };
+                mx = team.across(team.reduce(mx, op), op);
+                if (mx > (W)-INFINITY) m_out = mx;  // else all of it is closed, and stays 0
+                const auto ex = scaler(m_out, heat, team.table());
+                s.out = team.across(team.reduce(worker ? sum_up(ex) : 0.0, add), add);
+            }
+            const double z_out = ((double)m_out - (double)m) * heat.inv;  // log of what s.out is a multiple of
             if (!(qr > 0.0 && s.out > 0.0) && qr == qr && s.out == s.out) qr = 0.0;
             if (worker && g) {
                 const double one_over = 1.0 / total, mass = sum_q + qr, c = empty ? 0.0 : scale * w * heat.t;
                 double a = c * mass * one_over;
                 const double a_in = empty ? 0.0 : a;
+                if (z_out != 0.0) a *= exp(z_out);
                 if (qr != 0.0) a -= c * qr / s.out;
                 const W a_out = empty ? (W)0 : (W)a;
-                const auto ex = scaler(m, heat, team.table());
+                const auto ex = scaler(m_out, heat, team.table());
 #pragma unroll UNROLL
                 for (int v = v0 + lane; v < v1; v += 32) {
                     Vec<T> x = sl.get(v);
@@ -375,7 +411,7 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT + 32, NT == kBl
             }
             if (helper && lane == 0 && team.part == 0) {
                 double loss = sum_qlq - s.qz + sum_q * log(total);
-                if (qr != 0.0) loss += qr * log(qr * total / s.out);
+                if (qr != 0.0) loss += qr * (log(qr * total / s.out) - z_out);
                 row_loss[row] = empty ? (W)0 : (W)(heat.t * heat.t * loss);
             }
         } else {  // for every block of a cluster alike

@@ -602,7 +602,8 @@ int hx_top_logits_dev(hx_ctx* ctx, const hx_readout* rows, int k, double tempera
  *     q_r = max(0, 1 - sum q_j), p_r = sum of p outside the slots,
  *     L = T^2 (sum_j q_j (log q_j - log p_j) + q_r (log q_r - log p_r)),
  *     dL/dx_i = T (Q p_i - q_i) in a slot and T p_i (Q - q_r / p_r) outside,
- *     Q = sum q_j + q_r; a term whose q is 0, or whose p_r is 0, is left out.
+ *     Q = sum q_j + q_r; a term whose q is 0 is left out, and the rest's where
+ *     no readout outside the slots is open.
  * row_loss_dev[r] = L_r; *loss_dev = scale * sum_r w_r L_r, with w =
  * row_weight_dev (nrow doubles) or 1; grad_dev (rows' type, row r at
  * grad_dev + r * ld_grad; may be NULL, or the rows' own memory with the same

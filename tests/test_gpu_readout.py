@@ -938,3 +938,52 @@ def test_nan_of_either_sign(sim, dtype):
             g, rl, lo = call_distill(sim, view, ld, record(order, val, lse if rest else None, "f64"), 1.0, dtype, "f64")
             assert np.isnan(rl[:2]).all() and np.isnan(wide(g[:2])).all() and math.isnan(lo)
             assert np.isfinite(rl[2:]).all() and torch.isfinite(g[2:]).all()
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("nrow,n", [(3, 40), (3, 700), (200, 5003), (3, 60001), (4000, 120)])
+def test_distill_rest_far_below_the_slots(sim, dtype, nrow, n):
+    """Rows whose readouts outside the slots lie further below than the types' exponents reach, in logarithms:
+    log p_r = max / T + log S' - log S is off by E (of S' and S) + 2^-50 |log p_r|; a share e' / S' by 2 E and 3 u |z|
+    (within E); q_r by N as above."""
+    rng = np.random.default_rng(n)
+    k, T, scale = 3, 0.5, 2.0
+    x = rng.integers(0, 8, (nrow, n)) * 0.25
+    gap = rng.choice([10.0, 21.0, 24.0, 40.0, 47.0, 60.0, 174.0, 360.0, 375.0, 1000.0], nrow)
+    order = np.argsort(rng.random((nrow, n)), axis=1)[:, :k]
+    r = np.arange(nrow)[:, None]
+    x[rng.random(x.shape) < 0.1] = -np.inf
+    x[r, order] = gap[:, None] + [2.0, 0.0, 1.0]
+    x[0, np.setdiff1d(np.arange(n), order[0])] = -np.inf  # nothing is open outside: no term
+    val = np.tile([1.0, 0.25, 0.5], (nrow, 1))
+    lse = val.max(1) / T + 1.0
+    buf, view, ld = place(x, dtype)
+    xx, rec = wide(view), record(order, val, lse, "f64")
+    g, rl, lo = call_distill(sim, view, ld, rec, T, dtype, "f64", scale=scale)
+    g = wide(g)
+    noise = 2.0**-50 * (k + 8 + np.abs(val).max() / T)
+    with np.errstate(divide="ignore", invalid="ignore", over="ignore"):
+        for i in range(nrow):
+            a = np.zeros(n, bool)
+            a[order[i]] = True
+            z = (xx[i] - xx[i].max()) / T
+            logS = math.log(np.exp(z).sum())
+            lq = val[i] / T - lse[i]
+            q, lp = np.exp(lq), z[order[i]] - logS
+            qr = 1.0 - q.sum()
+            top = z[~a].max()
+            E = row_error(xx[i][a], T, dtype) + (row_error(xx[i][~a], T, dtype) if top > -np.inf else 0.0)
+            L, dL = (q * (lq - lp)).sum(), (q * (E + noise * (2 + np.abs(lq - lp) + np.abs(lp)))).sum()
+            if top > -np.inf:
+                e = np.where(a, 0.0, np.exp(z - top))
+                share, lpr = e / e.sum(), top + math.log(e.sum()) - logS
+                L += qr * (math.log(qr) - lpr)
+                dL += 2 * E * qr + noise * (abs(math.log(qr)) + 2 * abs(lpr) + 2)
+            else:
+                share, qr = np.zeros(n), 0.0
+            c, p = scale * T, np.exp(z - logS)
+            G = c * ((q.sum() + qr) * p - qr * share)
+            G[order[i]] -= c * q
+            dG = c * ((p + share) * (2 * E + 3 * noise) + np.where(a, noise, 0.0)) + np.abs(G) * HALF[dtype] * (1 + 2.0**-20) + TINY[dtype] * (1 + 2.0**-8)
+            assert abs(rl[i] - T * T * L) <= T * T * (dL + 2 * stat_u(dtype) * abs(L)), (i, gap[i], rl[i], T * T * L)
+            assert (np.abs(g[i] - G) <= dG).all(), (i, gap[i], np.abs(g[i] - G).max())
