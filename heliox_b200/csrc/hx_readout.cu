@@ -392,20 +392,27 @@ __global__ void __launch_bounds__(NT == 32 ? 32 * kWarpRows : NT + 32, NT == kBl
                 const double a_in = empty ? 0.0 : a;
                 if (z_out != 0.0) a *= exp(z_out);
                 if (qr != 0.0) a -= c * qr / s.out;
-                const W a_out = empty ? (W)0 : (W)a;
+                if (empty) a = 0.0;
                 const auto ex = scaler(m_out, heat, team.table());
+                const auto times = [&](const auto by) {  // the exponentials times a, in the type of `by`
 #pragma unroll UNROLL
-                for (int v = v0 + lane; v < v1; v += 32) {
-                    Vec<T> x = sl.get(v);
+                    for (int v = v0 + lane; v < v1; v += 32) {
+                        Vec<T> x = sl.get(v);
 #pragma unroll
-                    for (int u = 0; u < VEC; u++) {
-                        if constexpr (sizeof(T) == sizeof(W))
-                            x.e[u] = x.e[u] * a_out;
-                        else
-                            x.e[u] = narrow<T>(ex(wide(x.e[u])) * a_out);
+                        for (int u = 0; u < VEC; u++) {
+                            if constexpr (sizeof(T) == sizeof(W))
+                                x.e[u] = (W)(x.e[u] * by);
+                            else
+                                x.e[u] = narrow<T>((W)(ex(wide(x.e[u])) * by));
+                        }
+                        sl.set(v, x);
                     }
-                    sl.set(v, x);
-                }
+                };
+                // a large or a tiny scale's factor may be beyond fp32 where the products are not
+                if (sizeof(W) == 8 || a == 0.0 || !(fabs(a) < 0x1p-126 || fabs(a) > 0x1p127))
+                    times((W)a);
+                else
+                    times(a);
                 __syncwarp();
                 slots.each(sl, k, v0, v1, [&](int j, T* cell) { *cell = narrow<T>((W)(a_in * slots.x[j] - c * slots.q[j])); });
             }

@@ -987,3 +987,32 @@ def test_distill_rest_far_below_the_slots(sim, dtype, nrow, n):
             dG = c * ((p + share) * (2 * E + 3 * noise) + np.where(a, noise, 0.0)) + np.abs(G) * HALF[dtype] * (1 + 2.0**-20) + TINY[dtype] * (1 + 2.0**-8)
             assert abs(rl[i] - T * T * L) <= T * T * (dL + 2 * stat_u(dtype) * abs(L)), (i, gap[i], rl[i], T * T * L)
             assert (np.abs(g[i] - G) <= dG).all(), (i, gap[i], np.abs(g[i] - G).max())
+
+
+@pytest.mark.parametrize("dtype", ["f64", "f32", "bf16"])
+@pytest.mark.parametrize("n", [40, 700, 9000])
+def test_distill_factors_beyond_fp32(sim, dtype, n):
+    # products within the type's range whose factors are not: a loss scale of 1e27 with a rest e^-41 below, one of 1e-32 with
+    # slots e^-25 below; errors as for every gradient, relative to the shares
+    rng = np.random.default_rng(n)
+    h = HALF[dtype]
+    x = np.full((1, n), 1.0) + rng.integers(0, 4, (1, n)) * 0.25
+    x[0, 3], x[0, 7] = 42.0, -np.inf
+    buf, view, ld = place(x, dtype)
+    g, rl, lo = call_distill(sim, view, ld, record(np.array([[3]]), np.zeros((1, 1)), np.array([0.5]), "f64"), 1.0, dtype, "f64", scale=1e27)
+    z = wide(view)[0] - 42.0
+    out, qr = np.where(np.arange(n) == 3, 0.0, np.exp(z)), 1.0 - math.exp(-0.5)
+    p = np.exp(z) / np.exp(z).sum()
+    G = 1e27 * np.where(np.arange(n) == 3, p - math.exp(-0.5), p - qr * out / out.sum())
+    got = wide(g[0])
+    assert got[7] == 0.0 and (np.abs(got - G) <= (h + 2 * row_error(wide(view)[0], 1.0, dtype)) * (np.abs(G) + 1e27 * p)).all()
+
+    x = rng.integers(0, 8, (1, n)) * 0.25
+    x[0, 5] = -25.0
+    buf, view, ld = place(x, dtype)
+    g, rl, lo = call_distill(sim, view, ld, record(np.array([[5]]), np.zeros((1, 1)), None, "f64"), 1.0, dtype, "f64", scale=1e-32)
+    z = wide(view)[0] - wide(view)[0].max()
+    p = np.exp(z) / np.exp(z).sum()
+    G = 1e-32 * (p - (np.arange(n) == 5))
+    got = wide(g[0])
+    assert (np.abs(got - G) <= (h + 2 * row_error(wide(view)[0], 1.0, dtype)) * np.abs(G)).all()
