@@ -1016,3 +1016,20 @@ def test_distill_factors_beyond_fp32(sim, dtype, n):
     G = 1e-32 * (p - (np.arange(n) == 5))
     got = wide(g[0])
     assert (np.abs(got - G) <= (h + 2 * row_error(wide(view)[0], 1.0, dtype)) * np.abs(G)).all()
+
+
+def test_distill_as_many_rows_as_an_int_counts(sim):
+    # 30 GB: every row's loss is log 2, the last one's log(1 + e)
+    nrow = 2**31 - 1
+    x = torch.zeros((nrow, 2), dtype=torch.bfloat16, device="cuda")
+    x[-1, 1] = 1.0
+    ti, tv = torch.zeros((nrow, 1), dtype=torch.int32, device="cuda"), torch.zeros((nrow, 1), dtype=torch.bfloat16, device="cuda")
+    rl, lo = torch.zeros(nrow, dtype=torch.float32, device="cuda"), torch.zeros(1, dtype=torch.float32, device="cuda")
+    sim.distill_loss_grad_dev(x.data_ptr(), nrow, 2, 1, ti.data_ptr(), tv.data_ptr(), 0, rl.data_ptr(), lo.data_ptr(), dtype="bf16")
+    torch.cuda.synchronize()
+    u = 2.0**-24
+    assert abs(float(rl[-1]) - math.log(1 + math.e)) <= 40 * u
+    assert abs(float(rl[:-1].min()) - math.log(2)) <= 40 * u and abs(float(rl[:-1].max()) - math.log(2)) <= 40 * u
+    assert abs(float(lo[0]) - math.log(2)) <= 40 * u  # their mean
+    del x, ti, tv, rl
+    torch.cuda.empty_cache()
