@@ -124,3 +124,30 @@ def test_python_dtype_names():
     with pytest.raises(ValueError, match="dtype"):
         _readout(0, 1, 2, "float64", None)
     assert {"top_logits_dev", "distill_loss_grad_dev", "sample_dev"} <= set(dir(Sim))
+
+
+def test_python_numbers_that_do_not_fit():
+    # a descriptor's int would cut 2^32 + 3 rows to 3, and answer for those
+    for kw, word in ((dict(nrow=2**32 + 3), "nrow"), (dict(nrow=2**31), "nrow"), (dict(ncol=2**32 + 2), "ncol"), (dict(ld=2**64 + 2), "ld"),
+                     (dict(nrow=-(2**32) + 1), "nrow")):
+        with pytest.raises(ValueError, match=word):
+            _readout(**{**dict(ptr=P, nrow=1, ncol=2, dtype="f64", ld=None), **kw})
+    assert _readout(P, 2**31 - 1, 2, "f64", 2**40).ld == 2**40
+
+    class Lib:
+        def __getattr__(self, name):
+            def called(*args):
+                raise AssertionError(name)
+
+            return called
+
+    s = Sim.__new__(Sim)
+    s._L, s._ctx = Lib(), None
+    with pytest.raises(ValueError, match="^k "):
+        s.top_logits_dev(P, 1, 2, 2**32 + 1, P, P)
+    with pytest.raises(ValueError, match="^k "):
+        s.distill_loss_grad_dev(P, 1, 2, 2**32 + 1, P, P, P, P, P)
+    with pytest.raises(ValueError, match="ld_grad"):
+        s.distill_loss_grad_dev(P, 1, 2, 1, P, P, P, P, P, ld_grad=2**64 + 2)
+    with pytest.raises(ValueError, match="nrow"):
+        s.sample_dev(P, 2**32 + 1, 2, P, P)
