@@ -478,13 +478,15 @@ int type_size(int dtype) { return dtype == HX_DT_F64 ? 8 : dtype == HX_DT_F32 ? 
 int stat_size(int dtype) { return dtype == HX_DT_F64 ? 8 : 4; }
 bool off(const void* p, int align) { return (size_t)p % (size_t)align != 0; }
 
+constexpr long long kMostElements = 1ll << 56;  // of rows and what lies between them: no address space has more, and byte offsets fit 64 bits
+
 const char* check_rows(const hx_readout* r) {
     if (!r) return "null rows";
     if (r->dtype < HX_DT_F64 || r->dtype > HX_DT_BF16) return "rows: unknown dtype";
     if (r->nrow < 0 || r->ncol < 0) return "rows: nrow and ncol must not be negative";
     if (r->ld < r->ncol) return "rows: ld must be at least ncol";
     if ((long long)r->ncol * type_size(r->dtype) > HX_READOUT_MAX_ROW_BYTES) return "rows: a row is longer than HX_READOUT_MAX_ROW_BYTES";
-    if (r->nrow > 1 && r->ld > (1ll << 60) / r->nrow) return "rows: ld is out of range";
+    if (r->nrow > 1 && r->ld > kMostElements / r->nrow) return "rows: ld is out of range";
     if (r->nrow > 0 && r->ncol > 0 && !r->x) return "rows: null x";
     if (off(r->x, type_size(r->dtype))) return "rows: x is not aligned to its type";
     return nullptr;
@@ -517,7 +519,7 @@ const char* check_distill(const hx_readout* r, const hx_teacher* t, double tempe
         return "an array is not aligned to its type";
     if (!grad || r->nrow == 0 || r->ncol == 0) return nullptr;
     if (ldg < r->ncol) return "ld_grad must be at least ncol";
-    if (r->nrow > 1 && ldg > (1ll << 60) / r->nrow) return "ld_grad is out of range";
+    if (r->nrow > 1 && ldg > kMostElements / r->nrow) return "ld_grad is out of range";
     if (grad == r->x) return r->nrow == 1 || ldg == r->ld ? nullptr : "grad in place of x needs the same ld";
     // other overlaps: rows between rows are apart, everything else is refused
     const long long es = type_size(r->dtype);

@@ -151,3 +151,13 @@ def test_python_numbers_that_do_not_fit():
         s.distill_loss_grad_dev(P, 1, 2, 1, P, P, P, P, P, ld_grad=2**64 + 2)
     with pytest.raises(ValueError, match="nrow"):
         s.sample_dev(P, 2**32 + 1, 2, P, P)
+
+
+def test_offsets_beyond_any_address():
+    # nrow * ld elements whose bytes do not fit 64 bits, in the rows and in the gradient
+    for nrow, ld in ((1 << 20, 1 << 40), (1 << 16, 1 << 42), (2, 1 << 59)):
+        for rc, msg in (top(rows(nrow=nrow, ld=ld)), distill(rows(nrow=nrow, ld=ld), ldg=ld), sample(rows(nrow=nrow, ld=ld))):
+            assert rc == -1 and "ld is out of range" in msg
+        rc, msg = distill(rows(nrow=nrow), ldg=ld)
+        assert rc == -1 and "ld_grad is out of range" in msg
+    assert distill(rows(nrow=1 << 16, ld=1 << 40), ldg=1 << 40, grad=P + 80)[0] == 0
