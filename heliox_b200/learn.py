@@ -14,6 +14,7 @@ through ``Sim.optimizer_*`` (SimWrapper.cpp:284-451), run on the device.
 """
 from __future__ import annotations
 
+from contextlib import contextmanager
 from dataclasses import dataclass, field
 from typing import Any, Callable, Dict, List, Optional, Protocol, Sequence, Tuple, runtime_checkable
 
@@ -233,6 +234,16 @@ def _device_trace(runtime: AdjointRuntime, total_steps: int, ncol: int):
     return buf
 
 
+@contextmanager
+def _settled(sim: Sim):
+    """Leaves the block, also by an exception, with the context's work done: until
+    then it uses torch's buffers, which torch would give to others."""
+    try:
+        yield
+    finally:
+        sim.synchronize()
+
+
 def record_teacher(runtime: AdjointRuntime, total_steps: int, k: int, temperature: float = 1.0, rest: bool = True,
                    probes: Optional[Sequence[int]] = None) -> TeacherRecord:
     """Run a teacher and keep the ``k`` largest readouts of every step.
@@ -251,10 +262,10 @@ def record_teacher(runtime: AdjointRuntime, total_steps: int, k: int, temperatur
     idx = torch.empty((T, int(k)), dtype=torch.int32, device=trace.device)
     val = torch.empty((T, int(k)), dtype=torch.float64, device=trace.device)
     lse = torch.empty(T, dtype=torch.float64, device=trace.device) if rest else None
-    sim.forward_capture_dev(T, trace.data_ptr(), probes=p)
-    sim.top_logits_dev(trace[1:].data_ptr(), T, n, int(k), idx.data_ptr(), val.data_ptr(),
-                       lse_ptr=0 if lse is None else lse.data_ptr(), temperature=temperature)
-    sim.synchronize()
+    with _settled(sim):
+        sim.forward_capture_dev(T, trace.data_ptr(), probes=p)
+        sim.top_logits_dev(trace[1:].data_ptr(), T, n, int(k), idx.data_ptr(), val.data_ptr(),
+                           lse_ptr=0 if lse is None else lse.data_ptr(), temperature=temperature)
     return TeacherRecord(idx, val, lse, n, float(temperature))
 
 
@@ -288,19 +299,19 @@ def train_distill(runtime: AdjointRuntime, handles: Sequence[int], teacher: Teac
     sim.optimizer_add_external_grads(opt, list(handles), impedance=1.0)
     if allreduce is not None:
         sim.optimizer_set_allreduce(opt, allreduce)
-    for ep in range(int(epochs)):
-        sim.forward_capture_dev(T, trace.data_ptr(), probes=p)
-        sim.distill_loss_grad_dev(trace[1:].data_ptr(), T, n, teacher.k, teacher.idx.data_ptr(), teacher.val.data_ptr(),
-                                  dLdv[1:].data_ptr(), row_loss.data_ptr(), losses[ep:].data_ptr(),
-                                  t_lse_ptr=0 if teacher.lse is None else teacher.lse.data_ptr(),
-                                  temperature=teacher.temperature, row_weight_ptr=0 if w is None else w.data_ptr())
-        sim.backward_dev(dLdv.data_ptr(), {})
-        sim.optimizer_grads_from_backward(opt)
-        sim.optimizer_step_with_inv_record_steps(opt, lr, 1.0)
-        if on_epoch:
-            sim.synchronize()
-            on_epoch(ep, float(losses[ep]))
-    sim.synchronize()
+    with _settled(sim):
+        for ep in range(int(epochs)):
+            sim.forward_capture_dev(T, trace.data_ptr(), probes=p)
+            sim.distill_loss_grad_dev(trace[1:].data_ptr(), T, n, teacher.k, teacher.idx.data_ptr(), teacher.val.data_ptr(),
+                                      dLdv[1:].data_ptr(), row_loss.data_ptr(), losses[ep:].data_ptr(),
+                                      t_lse_ptr=0 if teacher.lse is None else teacher.lse.data_ptr(),
+                                      temperature=teacher.temperature, row_weight_ptr=0 if w is None else w.data_ptr())
+            sim.backward_dev(dLdv.data_ptr(), {})
+            sim.optimizer_grads_from_backward(opt)
+            sim.optimizer_step_with_inv_record_steps(opt, lr, 1.0)
+            if on_epoch:
+                sim.synchronize()
+                on_epoch(ep, float(losses[ep]))
     return [float(x) for x in losses[:int(epochs)].cpu()]
 
 
@@ -323,8 +334,8 @@ def sample_choices(runtime: AdjointRuntime, total_steps: int, u: np.ndarray, tem
     idx = torch.empty(m, dtype=torch.int32, device=trace.device)
     logp = torch.empty(m, dtype=torch.float64, device=trace.device)
     torch.cuda.current_stream(trace.device).synchronize()
-    sim.forward_capture_dev(T, trace.data_ptr(), probes=p)
-    sim.sample_dev(trace[T + 1 - m:].data_ptr(), m, n, ud.data_ptr(), idx.data_ptr(), logp_ptr=logp.data_ptr(),
-                   temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
-    sim.synchronize()
+    with _settled(sim):
+        sim.forward_capture_dev(T, trace.data_ptr(), probes=p)
+        sim.sample_dev(trace[T + 1 - m:].data_ptr(), m, n, ud.data_ptr(), idx.data_ptr(), logp_ptr=logp.data_ptr(),
+                       temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
     return idx.cpu().numpy(), logp.cpu().numpy()
