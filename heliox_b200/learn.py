@@ -207,11 +207,12 @@ def train_adam(runtime: AdjointRuntime, handles: Sequence[int], target: np.ndarr
 @dataclass
 class TeacherRecord:
     """A teacher's top readouts of the steps 1..T of a trial (device tensors):
-    what ``train_distill`` fits a student to."""
+    what ``train_distill`` fits a student to.  ``record_teacher`` keeps those of a
+    network; those of another model, or labels, may be put together by hand."""
 
     idx: Any  # int32 (T, k): probe columns in descending order, -1 where unused
-    val: Any  # float64 (T, k): their voltages
-    lse: Any  # float64 (T,) log-sum-exp of the whole row at ``temperature``, or None
+    val: Any  # float64, float32, float16 or bfloat16 (T, k): their voltages (or logits)
+    lse: Any  # (T,) log-sum-exp of the whole row at ``temperature`` (float64, float32 beside narrower val), or None
     ncol: int
     temperature: float
 
@@ -269,6 +270,31 @@ def record_teacher(runtime: AdjointRuntime, total_steps: int, k: int, temperatur
     return TeacherRecord(idx, val, lse, n, float(temperature))
 
 
+def _record_arrays(teacher: TeacherRecord, device):
+    """(idx, val, lse, type name of val) of a record as the library reads it."""
+    import torch
+
+    names = {torch.float64: "f64", torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"}
+    idx, val, lse = teacher.idx, teacher.val, teacher.lse
+    for what, x in (("idx", idx), ("val", val), ("lse", lse)):
+        if x is not None and x.device != device:
+            raise ValueError(f"the teacher's record is on {x.device} ({what}), the student on {device}")
+    if idx.dtype != torch.int32:
+        raise TypeError(f"the record's idx must be int32 (got {idx.dtype})")
+    if val.dtype not in names:
+        raise TypeError(f"the record's val must be float64, float32, float16 or bfloat16 (got {val.dtype})")
+    if idx.ndim != 2 or val.shape != idx.shape:
+        raise ValueError(f"the record's idx and val must both be (T, k) (got {tuple(idx.shape)} and {tuple(val.shape)})")
+    if lse is not None:
+        stat = torch.float64 if val.dtype == torch.float64 else torch.float32
+        if lse.dtype != stat:
+            raise TypeError(f"the record's lse must be {stat} beside {val.dtype} val (got {lse.dtype})")
+        if lse.shape != idx.shape[:1]:
+            raise ValueError(f"the record's lse must be (T,) (got {tuple(lse.shape)} beside {tuple(idx.shape)})")
+        lse = lse.contiguous()
+    return idx.contiguous(), val.contiguous(), lse, names[val.dtype]
+
+
 def train_distill(runtime: AdjointRuntime, handles: Sequence[int], teacher: TeacherRecord, epochs: int,
                   lr: float = 1e-3, probes: Optional[Sequence[int]] = None, row_weight: Optional[np.ndarray] = None,
                   allreduce: Optional[Callable[[int, int, int], None]] = None,
@@ -289,8 +315,7 @@ def train_distill(runtime: AdjointRuntime, handles: Sequence[int], teacher: Teac
     if row_weight is not None and np.shape(row_weight) != (T,):
         raise ValueError(f"row_weight must have shape ({T},)")
     trace, dLdv = _device_trace(runtime, T, n), _device_trace(runtime, T, n)  # row 0, the initial state, has no loss
-    if teacher.idx.device != trace.device:
-        raise ValueError(f"the teacher's record is on {teacher.idx.device}, the student on {trace.device}")
+    t_idx, t_val, t_lse, t_dtype = _record_arrays(teacher, trace.device)
     row_loss = torch.empty(T, dtype=torch.float64, device=trace.device)
     losses = torch.zeros(max(int(epochs), 1), dtype=torch.float64, device=trace.device)
     w = None if row_weight is None else torch.from_numpy(np.ascontiguousarray(row_weight, dtype=np.float64)).to(trace.device)
@@ -302,9 +327,9 @@ def train_distill(runtime: AdjointRuntime, handles: Sequence[int], teacher: Teac
     with _settled(sim):
         for ep in range(int(epochs)):
             sim.forward_capture_dev(T, trace.data_ptr(), probes=p)
-            sim.distill_loss_grad_dev(trace[1:].data_ptr(), T, n, teacher.k, teacher.idx.data_ptr(), teacher.val.data_ptr(),
+            sim.distill_loss_grad_dev(trace[1:].data_ptr(), T, n, teacher.k, t_idx.data_ptr(), t_val.data_ptr(),
                                       dLdv[1:].data_ptr(), row_loss.data_ptr(), losses[ep:].data_ptr(),
-                                      t_lse_ptr=0 if teacher.lse is None else teacher.lse.data_ptr(),
+                                      t_lse_ptr=0 if t_lse is None else t_lse.data_ptr(), t_dtype=t_dtype,
                                       temperature=teacher.temperature, row_weight_ptr=0 if w is None else w.data_ptr())
             sim.backward_dev(dLdv.data_ptr(), {})
             sim.optimizer_grads_from_backward(opt)

@@ -142,3 +142,21 @@ def test_train_distill_refuses_other_shapes():
     hist = train_distill(rt, h, rec, 3, probes=[0, 1, 2])
     assert len(hist) == 3 and np.isfinite(hist).all()
     rt.close()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_narrow_teachers_record_trains(dtype):
+    from heliox_b200.learn import AdjointRuntime, TeacherRecord, record_teacher, train_distill
+
+    g, gt = student_and_teacher()
+    rt = AdjointRuntime(gt)
+    rec = record_teacher(rt, T, K, TEMP)
+    rt.close()
+    val = rec.val.to(getattr(torch, dtype))
+    narrow = TeacherRecord(rec.idx, val, torch.zeros((T, 2), device="cuda", dtype=torch.float32).add_(rec.lse.float()[:, None])[:, 0], rec.ncol, TEMP)
+    st = AdjointRuntime(g)
+    trace = st.sim.forward_capture(T)
+    loss, _ = plain_loss_and_grad(trace, narrow, np.ones(T))
+    hist = train_distill(st, [st.handle("hh", "gnabar", 0)], narrow, 1)
+    assert abs(hist[0] - loss) <= 1e-9 * abs(loss)
+    st.close()

@@ -62,3 +62,42 @@ def test_work_is_done_at_the_end(run):
     rt = Runtime()
     RUNS[run](rt)
     assert rt.sim.calls[-1] == "synchronize"
+
+
+I32, F64, F32, F16, BF16 = torch.int32, torch.float64, torch.float32, torch.float16, torch.bfloat16
+
+
+@pytest.mark.parametrize("change,error,word", [
+    (dict(idx=torch.zeros((5, 2), dtype=torch.int64)), TypeError, "int32"),
+    (dict(val=torch.zeros((5, 2), dtype=torch.int32)), TypeError, "float64"),
+    (dict(val=torch.zeros((5, 2), dtype=F32)), TypeError, "lse must be torch.float32"),
+    (dict(lse=torch.zeros(5, dtype=F32)), TypeError, "lse must be torch.float64"),
+    (dict(val=torch.zeros((5, 2), dtype=BF16), lse=torch.zeros(5, dtype=BF16)), TypeError, "lse must be torch.float32"),
+    (dict(val=torch.zeros((5, 1), dtype=F64)), ValueError, r"\(T, k\)"),
+    (dict(val=torch.zeros((4, 2), dtype=F64)), ValueError, r"\(T, k\)"),
+    (dict(idx=torch.zeros(5, dtype=I32), val=torch.zeros(5, dtype=F64)), ValueError, r"\(T, k\)"),
+    (dict(lse=torch.zeros(4, dtype=F64)), ValueError, r"\(T,\)"),
+    (dict(lse=torch.zeros((5, 1), dtype=F64)), ValueError, r"\(T,\)"),
+    (dict(lse=torch.zeros(5, dtype=F64, device="meta")), ValueError, "is on meta"),
+])
+def test_records_that_the_library_would_misread(change, error, word):
+    rec = a_record()
+    for name, x in change.items():
+        setattr(rec, name, x)
+    rt = Runtime()
+    with pytest.raises(error, match=word):
+        learn.train_distill(rt, [0], rec, 1, probes=[0, 1, 2])
+    assert "distill_loss_grad_dev" not in rt.sim.calls
+
+
+@pytest.mark.parametrize("dtype,name", [(F64, "f64"), (F32, "f32"), (F16, "f16"), (BF16, "bf16")])
+def test_records_of_narrow_teachers_and_strided_ones(dtype, name):
+    rec = learn.TeacherRecord(torch.arange(10, dtype=I32).reshape(2, 5).T, torch.arange(20, dtype=dtype).reshape(5, 4)[:, ::2],
+                              torch.zeros((5, 2), dtype=F64 if dtype == F64 else F32)[:, 0], 3, 2.0)
+    idx, val, lse, got = learn._record_arrays(rec, torch.device("cpu"))
+    assert got == name and torch.equal(idx, rec.idx) and torch.equal(val, rec.val) and torch.equal(lse, rec.lse)
+    assert idx.is_contiguous() and val.is_contiguous() and lse.is_contiguous()
+    rt = Runtime()
+    learn.train_distill(rt, [0], rec, 1, probes=[0, 1, 2])
+    args, kw = rt.sim.kw["distill_loss_grad_dev"]
+    assert kw["t_dtype"] == name and args[3] == 2 and kw["t_lse_ptr"]
