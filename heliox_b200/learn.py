@@ -225,6 +225,12 @@ class TeacherRecord:
         return int(self.idx.shape[1])
 
 
+def _whole_network(sim: Sim, what: str) -> Sim:
+    if sim.sharded:
+        raise ValueError(f"{what} of a sharded network: the choice is among the probes of one rank's shard, not of the network")
+    return sim
+
+
 def _device_trace(runtime: AdjointRuntime, total_steps: int, ncol: int):
     """A zeroed (T+1, ncol) float64 buffer on the runtime's device, safe to use on the runtime's stream."""
     import torch
@@ -252,11 +258,13 @@ def record_teacher(runtime: AdjointRuntime, total_steps: int, k: int, temperatur
     The probes are the choices: step t's probabilities are softmax(v[t] /
     temperature) (temperature in mV).  ``rest`` also keeps each row's
     log-sum-exp, so that the loss counts what the k readouts leave out as one
-    more class; without it the k are renormalised.  A full float64 trace of
+    more class; without it the k are renormalised.  A row is the readouts of one
+    ``Sim``: a network that is sharded by cell over ranks is refused, here and
+    in ``train_distill`` and ``sample_choices``.  A full float64 trace of
     10,000 probes over 8,000 steps is 640 MB, 64 readouts of each step 6 MB."""
     import torch
 
-    sim = runtime.sim
+    sim = _whole_network(runtime.sim, "the record")
     p = runtime.group.soma_nodes() if probes is None else np.asarray(probes, dtype=np.int32)
     T, n = int(total_steps), int(len(p))
     trace = _device_trace(runtime, T, n)
@@ -304,10 +312,11 @@ def train_distill(runtime: AdjointRuntime, handles: Sequence[int], teacher: Teac
     ``train_adam`` with the distillation loss in place of the trace's MSE, the
     mean over the teacher's steps: forward capture, loss and gradient, reverse
     sweep and Adam all stay on the device.  ``row_weight`` (T): the weight of
-    each step, 0 leaves one out.  Returns the loss history."""
+    each step, 0 leaves one out.  ``allreduce``: of data-parallel replicas, as in
+    ``train_adam``.  Returns the loss history."""
     import torch
 
-    sim = runtime.sim
+    sim = _whole_network(runtime.sim, "distillation")
     p = runtime.group.soma_nodes() if probes is None else np.asarray(probes, dtype=np.int32)
     T, n = teacher.total_steps, teacher.ncol
     if len(p) != n:
@@ -347,7 +356,7 @@ def sample_choices(runtime: AdjointRuntime, total_steps: int, u: np.ndarray, tem
     log-probabilities float64)."""
     import torch
 
-    sim = runtime.sim
+    sim = _whole_network(runtime.sim, "choices")
     p = runtime.group.soma_nodes() if probes is None else np.asarray(probes, dtype=np.int32)
     T, n = int(total_steps), int(len(p))
     uu = np.ascontiguousarray(u, dtype=np.float64)

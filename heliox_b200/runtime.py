@@ -148,6 +148,11 @@ class Sim:
         self._bound = _lib.BoundGroup(group, gid_base=gid_base, nsrc_cells=nsrc_cells)
         self._check(self._L.hx_load_group(self._ctx, C.byref(self._bound.desc)), "hx_load_group")
 
+    @property
+    def sharded(self) -> bool:
+        """Whether the loaded group is one shard of a network that other ranks hold the rest of."""
+        return self.group is not None and self._bound.desc.nsrc_cells > self.group.ncell
+
     def plan_stats(self) -> dict:
         st = _lib.PlanStats()
         self._check(self._L.hx_get_plan_stats(self._ctx, C.byref(st)), "hx_get_plan_stats")

@@ -10,7 +10,7 @@ from heliox_b200 import learn  # noqa: E402
 
 class Sim:
     def __init__(self, refuse=None):
-        self.device, self.refuse, self.calls, self.kw = 0, refuse, [], {}
+        self.device, self.refuse, self.calls, self.kw, self.sharded = 0, refuse, [], {}, False
 
     def __getattr__(self, name):
         def call(*args, **kw):
@@ -101,3 +101,29 @@ def test_records_of_narrow_teachers_and_strided_ones(dtype, name):
     learn.train_distill(rt, [0], rec, 1, probes=[0, 1, 2])
     args, kw = rt.sim.kw["distill_loss_grad_dev"]
     assert kw["t_dtype"] == name and args[3] == 2 and kw["t_lse_ptr"]
+
+
+@pytest.mark.parametrize("run", list(RUNS))
+def test_a_sharded_network_is_refused(run):
+    rt = Runtime()
+    rt.sim.sharded = True
+    with pytest.raises(ValueError, match="sharded network"):
+        RUNS[run](rt)
+    assert rt.sim.calls == []
+
+
+def test_what_counts_as_sharded():
+    from heliox_b200 import _lib, runtime, shard, synth
+
+    s = runtime.Sim.__new__(runtime.Sim)
+    s.group = None
+    assert not s.sharded
+    g = synth.spiking_network(6)
+    s.group, s._bound = g, _lib.BoundGroup(g)
+    assert not s.sharded
+    part, base, nsrc = shard.shard(g, 2, 1)
+    s.group, s._bound = part, _lib.BoundGroup(part, gid_base=base, nsrc_cells=nsrc)
+    assert s.sharded
+    whole, base, nsrc = shard.shard(g, 1, 0)
+    s.group, s._bound = whole, _lib.BoundGroup(whole, gid_base=base, nsrc_cells=nsrc)
+    assert not s.sharded
