@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(kLossThreads) loss_kernel(const W* __restrict_
     __shared__ double red[32];
     double s = 0;
 #pragma unroll 8
-    for (long long r = threadIdx.x; r < nrow; r += kLossThreads) {  // up to 2^31 - 1 of them
+    for (unsigned r = threadIdx.x; r < (unsigned)nrow; r += kLossThreads) {  // up to 2^31 - 1 of them
         const double w = weight ? weight[r] : 1.0, l = (double)row_loss[r];
         s += w != 0.0 ? w * l : 0.0;
     }

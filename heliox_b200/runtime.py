@@ -85,17 +85,17 @@ def _dt(dtype: str) -> int:
     return _lib.HX_DT[dtype]
 
 
-def _c_int(name: str, n: int, bits: int = 32) -> int:
-    """``n`` as the C int (or long long) of a descriptor, which would cut it off silently."""
-    n = int(n)
-    if not -(1 << (bits - 1)) <= n < 1 << (bits - 1):
-        raise ValueError(f"{name} does not fit {bits} bits (got {n})")
-    return n
+def _too_large(**counts: int) -> ValueError:
+    return ValueError(", ".join(f"{k} = {v}" for k, v in counts.items()) + ": beyond the descriptor's ints")
 
 
 def _readout(ptr: int, nrow: int, ncol: int, dtype: str, ld: Optional[int]) -> "_lib.Readout":
-    return _lib.Readout(int(ptr) or None, _dt(dtype), _c_int("nrow", nrow), _c_int("ncol", ncol),
-                        _c_int("ld", ncol if ld is None else ld, 64))
+    """Counts that a C int (ld: a long long) would cut off are refused; negative ones by the library."""
+    nrow, ncol = int(nrow), int(ncol)
+    ld = ncol if ld is None else int(ld)
+    if (nrow | ncol) >> 31 not in (0, -1) or ld >> 63 not in (0, -1):
+        raise _too_large(nrow=nrow, ncol=ncol, ld=ld)
+    return _lib.Readout(int(ptr) or None, _dt(dtype), nrow, ncol, ld)
 
 
 class Sim:
@@ -400,7 +400,10 @@ class Sim:
         k int32; ``val_ptr``: nrow x k of ``dtype``; ``lse_ptr``: nrow values
         (float64 for "f64" rows, else float32), 0 to leave them out."""
         rows = _readout(logits_ptr, nrow, ncol, dtype, ld)
-        self._check(self._L.hx_top_logits_dev(self._ctx, C.byref(rows), _c_int("k", k), float(temperature),
+        k = int(k)
+        if k >> 31 not in (0, -1):
+            raise _too_large(k=k)
+        self._check(self._L.hx_top_logits_dev(self._ctx, C.byref(rows), k, float(temperature),
                                               int(idx_ptr), int(val_ptr),
                                               int(lse_ptr)), "hx_top_logits_dev")
 
@@ -419,12 +422,14 @@ class Sim:
         rows, else float32).  ``scale`` defaults to 1 / nrow (the mean over
         rows); ``row_weight_ptr``: nrow float64 weights, 0 for ones."""
         rows = _readout(logits_ptr, nrow, ncol, dtype, ld)
-        t = _lib.Teacher(int(t_idx_ptr), int(t_val_ptr), int(t_lse_ptr) or None, _dt(t_dtype or dtype),
-                         _c_int("k", k))
+        k, ld_grad = int(k), int(ncol if ld_grad is None else ld_grad)
+        if k >> 31 not in (0, -1) or ld_grad >> 63 not in (0, -1):
+            raise _too_large(k=k, ld_grad=ld_grad)
+        t = _lib.Teacher(int(t_idx_ptr), int(t_val_ptr), int(t_lse_ptr) or None, _dt(t_dtype or dtype), k)
         sc = (1.0 / nrow if nrow > 0 else 1.0) if scale is None else float(scale)
         self._check(self._L.hx_distill_loss_grad_dev(
             self._ctx, C.byref(rows), C.byref(t), float(temperature), sc, int(row_weight_ptr),
-            int(grad_ptr), _c_int("ld_grad", ncol if ld_grad is None else ld_grad, 64), int(row_loss_ptr),
+            int(grad_ptr), ld_grad, int(row_loss_ptr),
             int(loss_ptr)), "hx_distill_loss_grad_dev")
 
     def sample_dev(self, logits_ptr: int, nrow: int, ncol: int, u_ptr: int, idx_ptr: int, *, logp_ptr: int = 0,
