@@ -38,13 +38,14 @@ constexpr int kBlock = 256;  // threads of a block that has a row, or a slice of
 template <typename T>
 constexpr int kBlocks = sizeof(T) == 8 ? 2 : 3;  // such blocks on an SM, where their shared memory lets them
 
-// Measured (B200): 4000 x 10000 fp64 rows, 64 slots: 163 us, 3.9 TB/s of reads
+// Measured (B200): 4000 x 10000 fp64 rows, 64 slots: 168 us, 3.8 TB/s of reads
 // and writes, with two 80 KB rows an SM in flight and the warps' dependent
 // chains between them as the bound; 1021 x 32003 bf16 51 us; 8000 x 302 fp64,
 // a warp a row, 28 us, about 900 instructions a row besides its readouts.
 // Blocks of 512 threads: 199 us for the first, 62 for the second (each warp has
 // its share of reductions and divisions once a row); 3 blocks of 256 an SM
-// against 2: 50 and 55 us for the second.
+// against 2: 50 and 55 us for the second.  Without copying the next row to L2
+// ahead: 174 us against 167 for the first, 219 against 211 at 8000 x 3000.
 constexpr double kFar = 0x1p-64;  // a sum from here on has lost no readout that counts to the exponentials' range (2^-126 in fp32)
 constexpr int kFewSlots = 128;  // up to here the next row's slots are worked out into lists of their own
 

@@ -543,6 +543,7 @@ int hx_mse_loss_grad_noalloc(const double* trace_dev, const double* target_dev, 
  * another order).  A -inf readout is a closed choice: it has
  * probability 0 and is never taken.  "Statistics" (log-sum-exp, losses,
  * log-probabilities) are double for HX_DT_F64 rows and float for the others.
+ * Outputs overlap neither inputs nor one another, but for grad_dev as said there.
  * The reference has no counterpart (its objectives are Python callables on the
  * output trace, python_lib/heliox_learn/objective.py:15-30). */
 enum hx_dtype { HX_DT_F64 = 0, HX_DT_F32 = 1, HX_DT_F16 = 2, HX_DT_BF16 = 3 };
@@ -610,6 +611,8 @@ int hx_top_logits_dev(hx_ctx* ctx, const hx_readout* rows, int k, double tempera
  * ld) = scale * w_r dL_r/dx, each rounded once.  Rows of weight 0 are not read;
  * they, rows without a used slot and rows without an open readout get a loss
  * of 0 and gradients of 0.  NaN, or +inf, in another row gives NaN there.
+ * In fp32, fp16 and bf16 rows a readout with less than 2^-60 of its row, or of the
+ * row's rest, may get a gradient of 0.
  * loss_dev and row_loss_dev: statistics of the rows' type. */
 int hx_distill_loss_grad_dev(hx_ctx* ctx, const hx_readout* rows, const hx_teacher* teacher, double temperature,
                              double scale, const double* row_weight_dev, void* grad_dev, long long ld_grad,
