@@ -30,9 +30,10 @@ using namespace hxr;
 // their places), so that the sum over the rest is a sum of its own and not a
 // difference.  A rest that the record gives a share, but that lies e^-44 or more
 // below, is summed up again relative to its own largest readout, so that its
-// logarithm and its readouts' shares of it are right at any distance.  The teacher's side of the next row is worked out meanwhile: in
-// a block of many warps by a helper, which has no run, so that its chain of
-// dependent exponentials and reductions is waited for by nobody.
+// logarithm and its readouts' shares of it are right at any distance.  The
+// teacher's side of the next row is worked out meanwhile: in a block of many
+// warps by a helper, which has no run, so that its chain of dependent
+// exponentials and reductions is waited for by nobody.
 
 constexpr int kBlock = 256;  // threads of a block that has a row, or a slice of one, to itself (short rows: 128)
 template <typename T>
@@ -46,7 +47,7 @@ constexpr int kBlocks = sizeof(T) == 8 ? 2 : 3;  // such blocks on an SM, where 
 // its share of reductions and divisions once a row); 3 blocks of 256 an SM
 // against 2: 50 and 55 us for the second.  Without copying the next row to L2
 // ahead: 174 us against 167 for the first, 219 against 211 at 8000 x 3000.
-constexpr double kFar = 0x1p-64;  // a sum from here on has lost no readout that counts to the exponentials' range (2^-126 in fp32)
+constexpr double kFar = 0x1p-64;  // a sum from here on has lost nothing that counts to the exponentials' range (2^-126 in fp32)
 constexpr int kFewSlots = 128;  // up to here the next row's slots are worked out into lists of their own
 
 __host__ __device__ constexpr int slot_list(int k) { return (k + 3) / 4 * 4; }
